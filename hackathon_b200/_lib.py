@@ -50,6 +50,17 @@ class TensorC(C.Structure):
     _fields_ = [("name", C.c_char_p), ("data", C.c_void_p), ("numel", C.c_int64)]
 
 
+class SequencesC(C.Structure):
+    _fields_ = [("starts", C.c_void_p), ("slots", C.c_void_p), ("seqs", C.c_int32), ("tokens", C.c_int32),
+                ("state_rows", C.c_int32), ("longest", C.c_int32)]
+
+
+class ScanArgsC(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("ssm", "x", "b", "c", "dt", "a", "d", "z", "y")]
+                + [(n, C.c_int64) for n in ("ldx", "ldb", "ldc", "lddt", "ldz", "ldy")]
+                + [(n, C.c_int32) for n in ("rows", "heads", "size", "state", "dtype", "softplus")])
+
+
 _P = C.c_void_p
 _I32 = C.c_int32
 _I64 = C.c_int64
@@ -83,6 +94,14 @@ _SIGS = {
     "b2e_mamba2_step": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _P, _P]),
     "b2e_linear": (C.c_int, [_P, _I32, _I32, _I32, _P, _I32, _P, _I32, _I32, _P, _P, _P]),
     "b2e_linear_static": (C.c_int, [_P, _I32, _I32, _I32, _P, _I32, _P, _I32, _I32, _P, _P, _P]),
+    "b2e_seqops_device_error": (C.c_int, [_PI32]),
+    "b2e_rms_norm_fp8": (C.c_int, [_P, _I32, _I64, _P, _I32, _I64, _P, C.c_float, _I32, _I32, _P, _I64, _P, _P, _P, _P]),
+    "b2e_quantize_fp8": (C.c_int, [_P, _I32, _I64, _I32, _I32, _P, _I64, _P, _P]),
+    "b2e_quantize_fp8_weight": (C.c_int, [_P, _I32, _I64, _I32, _I32, _P, _I64, _P, _P]),
+    "b2e_fp8_linear": (C.c_int, [_P, _I64, _P, _I32, _I32, _P, _I64, _P, _I32, _P, _I32, _P, _I32, _I64, _P]),
+    "b2e_causal_conv": (C.c_int, [_P, _P, _P, _I32, _I64, _I32, _I32, _P, _P, _I32, _I32, _P, _I64, _P]),
+    "b2e_mamba2_scan_workspace": (C.c_int, [_P, _P, _PI64]),
+    "b2e_mamba2_scan": (C.c_int, [_P, _P, _P, _I64, _P]),
     "b2e_layer_create": (C.c_int, [_I32, C.POINTER(ModelConfigC), C.POINTER(EngineOptionsC), C.POINTER(TensorC),
                                    _I32, C.POINTER(_P)]),
     "b2e_layer_destroy": (None, [_P]),

@@ -136,7 +136,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 __device__ __forceinline__ float4 ld_stream(const float4* p) { return __ldcs(p); }
 __device__ __forceinline__ void st_stream(float4* p, float4 v) { __stcs(p, v); }
 
-inline int ceil_div(long a, long b) { return int((a + b - 1) / b); }
+__host__ __device__ inline int ceil_div(long a, long b) { return int((a + b - 1) / b); }
 
 // ------------------------------------------------------------ launches
 // The engine launches the kernels of a tower's chain with programmatic stream

@@ -1,0 +1,511 @@
+// 8-bit projection: e4m3 operands, float32 scales for each 128 columns of an
+// activation row and each 128 x 128 block of the weight.
+//
+//   y[m, n] = act( sum_g xs[m, g] ws[n / 128, g] * (sum_{k in g} x[m, k] w[n, k]) + bias[n] )
+//
+// The inner sum over a group's 128 products is four tcgen05.mma of kind f8f6f4
+// into a fresh TMEM accumulator (float32); the epilogue warps read it, multiply
+// by the two scales and add it to float32 registers while the next group's MMAs
+// run into the other accumulator. The products of e4m3 values are exact in
+// float32. One K step of the pipeline is one scale group: 128 bytes, one
+// swizzled row.
+//
+// Two shapes of the same pipeline:
+//  - rows kernel: M = 128 activation rows (a thread's TMEM lane is a row, so both
+//    scales are one scalar a thread and group), N = BN output features;
+//    persistent CTAs. Bound by the tensor cores: a group costs 128 x BN x 128
+//    products, its epilogue BN/2 FMAs a thread of eight warps.
+//  - few-rows kernel: M = 128 output features, N = BR <= 64 rows; the groups are
+//    shared out over a cluster of up to 8 CTAs, whose float32 sums meet through
+//    distributed shared memory in rank order (the same result every time). Bound
+//    by the weight's bytes.
+#include <algorithm>
+#include <cooperative_groups.h>
+
+#include "seqops.cuh"
+#include "tc.cuh"
+
+namespace b2e {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kEpi = 8;                       // epilogue warps
+constexpr int kThreads = 64 + 32 * kEpi;      // TMA warp, MMA warp, epilogue
+constexpr uint32_t kKB = kFp8Group;           // bytes of a K step
+enum Fp8Error : int { kFp8TimeoutTma = 121, kFp8TimeoutMma = 122, kFp8TimeoutEpi = 123 };
+
+// Instruction descriptor of kind f8f6f4: float32 accumulator, e4m3 x e4m3, both
+// K-major, M = 128, N = n.
+__host__ __device__ constexpr uint32_t idesc_f8(int n) {
+  return (1u << 4) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_f8(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+struct Args {
+  const float* xs;
+  const float* ws;
+  const float* bias;
+  void* y;
+  long long ldy;
+  int m, n, groups, wgroups;  // wgroups: scale columns of ws
+  int relu, y_type, vec;      // vec: rows of y may take 32-byte stores
+  int tiles_m, tiles_n;
+  int* err;
+};
+
+// Eight float results to a row of y, n % 8 == 0, all inside.
+__device__ __forceinline__ void store8_y(const Args& e, long long at, const float (&v)[8]) {
+  if (e.y_type == kF32) {
+    float* p = reinterpret_cast<float*>(e.y) + at;
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+                 "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+  } else {
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (e.y_type == kBF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        u[j] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        u[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(e.y) + at) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+// ------------------------------------------------------------- rows kernel
+
+template <int BN>
+struct RowsCfg {
+  static constexpr uint32_t TILE_X = 128 * kKB, TILE_W = BN * kKB, STAGE = TILE_X + TILE_W;
+  static constexpr int STAGES = BN == 256 ? 4 : 3;
+  static constexpr int CTAS = BN == 256 ? 1 : 2;  // resident on an SM
+  static constexpr uint32_t TMEM = 2 * BN;
+  static constexpr size_t SMEM = size_t(STAGES) * STAGE + 1024 + 256;
+};
+
+template <int BN>
+__global__ void __launch_bounds__(kThreads, RowsCfg<BN>::CTAS)
+    k_fp8_rows(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, const Args e) {
+  using K = RowsCfg<BN>;
+  constexpr int S = K::STAGES, HN = BN / 2;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + size_t(S) * K::STAGE);
+  uint64_t* empty = full + S;
+  uint64_t* pfull = empty + S;   // a group's sum is in TMEM buffer b
+  uint64_t* pempty = pfull + 2;  // its epilogue has read it
+  uint64_t* done = pempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&pfull[b], 1);
+      mbar_init(&pempty[b], kEpi);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+    tc::prefetch_map(&tx);
+    tc::prefetch_map(&tw);
+  }
+  if (warp == 1) tc::tmem_alloc(tmem_slot, K::TMEM);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int tiles = e.tiles_m * e.tiles_n;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      for (int t = blockIdx.x; t < tiles && !*abort_flag; t += gridDim.x) {
+        const int m0 = (t % e.tiles_m) * 128, n0 = (t / e.tiles_m) * BN;
+        for (int g = 0; g < e.groups; ++g, ++it) {
+          const int s = it % S;
+          if (it >= S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, abort_flag)) {
+            if (!*abort_flag) atomicExch(e.err, kFp8TimeoutTma);
+            *abort_flag = 1;
+            break;
+          }
+          uint8_t* st = smem + size_t(s) * K::STAGE;
+          mbar_expect_tx(&full[s], K::STAGE);
+          tc::tma_load_2d(st, &tx, g * int(kKB), m0, &full[s]);
+          tc::tma_load_2d(st + K::TILE_X, &tw, g * int(kKB), n0, &full[s]);
+        }
+      }
+      if (*abort_flag) {  // every load issued lands before the CTA leaves (bounded)
+        volatile int never = 0;
+        for (int i = max(0, it - S); i < it; ++i) mbar_wait(&full[i % S], (i / S) & 1, &never);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_f8(BN);
+      int it = 0;
+      for (int t = blockIdx.x; t < tiles && !*abort_flag; t += gridDim.x) {
+        for (int g = 0; g < e.groups; ++g, ++it) {
+          const int s = it % S, b = it & 1;
+          if ((it >= 2 && !mbar_wait(&pempty[b], ((it >> 1) & 1) ^ 1, abort_flag)) ||
+              !mbar_wait(&full[s], (it / S) & 1, abort_flag)) {
+            if (!*abort_flag) atomicExch(e.err, kFp8TimeoutMma);
+            *abort_flag = 1;
+            break;
+          }
+          tc::fence_after();
+          const uint32_t x0 = smem_u32(smem + size_t(s) * K::STAGE), w0 = x0 + K::TILE_X;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // K = 32 an instruction: 32 bytes further in the swizzled row
+            mma_f8(tmem + b * BN, tc::desc_k(x0 + k * 32), tc::desc_k(w0 + k * 32), idesc, k != 0);
+          tc::commit(&empty[s]);
+          tc::commit(&pfull[b]);
+        }
+      }
+      tc::commit(done);  // the CTA leaves (and frees its TMEM) after the last MMA
+      volatile int never = 0;
+      mbar_wait(done, 0, &never);
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lanes q*32.., columns half*HN..
+    int it = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+      const int m0 = (t % e.tiles_m) * 128, n0 = (t / e.tiles_m) * BN;
+      const int row = m0 + q * 32 + lane, c0 = n0 + half * HN;
+      const bool in = row < e.m;
+      const float* xs = e.xs + (long long)(in ? row : 0) * e.groups;
+      const float* ws = e.ws + (long long)(min(c0, e.n - 1) / kFp8Group) * e.wgroups;
+      float acc[HN];
+#pragma unroll
+      for (int j = 0; j < HN; ++j) acc[j] = 0.f;
+      float f = in ? xs[0] * ws[0] : 0.f;
+      bool ok = true;
+      for (int g = 0; g < e.groups; ++g, ++it) {
+        const int b = it & 1;
+        const float fn = in && g + 1 < e.groups ? xs[g + 1] * ws[g + 1] : 0.f;  // in flight beside this group
+        ok = mbar_wait(&pfull[b], (it >> 1) & 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) {
+          if (lane == 0 && !*abort_flag) atomicExch(e.err, kFp8TimeoutEpi);
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
+        tc::fence_after();
+#pragma unroll
+        for (int j = 0; j < HN; j += 32) {
+          uint32_t r[32];
+          tc::tmem_ld32(tmem + (uint32_t(q * 32) << 16) + uint32_t(b * BN + half * HN + j), r);
+          tc::tmem_wait_ld();
+          tc::landed(r);
+          if (j + 32 >= HN) {  // read: the next group but one may overwrite it
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pempty[b]);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[j + i] = fmaf(__uint_as_float(r[i]), f, acc[j + i]);
+        }
+        f = fn;
+      }
+      if (!ok) break;
+      if (in) {
+        const long long at = (long long)row * e.ldy + c0;
+#pragma unroll
+        for (int j = 0; j < HN; j += 8) {
+          if (c0 + j >= e.n) break;
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[i] = acc[j + i];
+            if (e.bias && c0 + j + i < e.n) v[i] += e.bias[c0 + j + i];
+            if (e.relu) v[i] = v[i] < 0.f ? 0.f : v[i];
+          }
+          if (e.vec && c0 + j + 8 <= e.n) {
+            store8_y(e, at + j, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c0 + j + i < e.n) store_as(e.y_type, e.y, size_t(at + j + i), v[i]);
+          }
+        }
+      }
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 1) tc::tmem_free(tmem, K::TMEM);
+}
+
+// --------------------------------------------------------- few-rows kernel
+
+constexpr int kFewStages = 8;
+constexpr int kFewThreads = 64 + 128;
+
+template <int BR>
+struct FewCfg {
+  static constexpr uint32_t TILE_W = 128 * kKB, TILE_X = BR * kKB, STAGE = TILE_W + TILE_X;
+  static constexpr uint32_t TMEM = 2 * BR < 32 ? 32 : 2 * BR;
+  // the ring; the float32 sums of the CTA's tile reuse it; then the row scales
+  static size_t smem(int stages, int local_groups) {
+    return 1024 + size_t(std::max(stages * int(STAGE), 128 * BR * 4)) + size_t(local_groups) * BR * 4 + 512;
+  }
+};
+
+template <int BR>
+__global__ void __launch_bounds__(kFewThreads)
+    k_fp8_few(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, const Args e, int stages) {
+  using K = FewCfg<BR>;
+  cg::cluster_group cl = cg::this_cluster();
+  const int nsplit = int(cl.num_blocks()), rank = int(cl.block_rank());
+  const int n0 = (blockIdx.x / nsplit) * 128, m0 = blockIdx.y * BR;
+  const int per = ceil_div(e.groups, nsplit), g0 = min(rank * per, e.groups), g1 = min(g0 + per, e.groups), ng = g1 - g0;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int ring = max(stages * int(K::STAGE), 128 * BR * 4);
+  float* xsc = reinterpret_cast<float*>(smem + ring);  // [group][row]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring + size_t(per) * BR * 4);
+  uint64_t* empty = full + kFewStages;
+  uint64_t* pfull = empty + kFewStages;
+  uint64_t* pempty = pfull + 2;
+  uint64_t* done = pempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&pfull[b], 1);
+      mbar_init(&pempty[b], 4);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+    tc::prefetch_map(&tx);
+    tc::prefetch_map(&tw);
+  }
+  if (warp == 1) tc::tmem_alloc(tmem_slot, K::TMEM);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+  float acc[BR];
+#pragma unroll
+  for (int j = 0; j < BR; ++j) acc[j] = 0.f;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      for (; it < ng; ++it) {
+        const int s = it % stages;
+        if (it >= stages && !mbar_wait(&empty[s], ((it / stages) & 1) ^ 1, abort_flag)) {
+          if (!*abort_flag) atomicExch(e.err, kFp8TimeoutTma);
+          *abort_flag = 1;
+          break;
+        }
+        uint8_t* st = smem + size_t(s) * K::STAGE;
+        mbar_expect_tx(&full[s], K::STAGE);
+        tc::tma_load_2d(st, &tw, (g0 + it) * int(kKB), n0, &full[s]);
+        tc::tma_load_2d(st + K::TILE_W, &tx, (g0 + it) * int(kKB), m0, &full[s]);
+      }
+      if (*abort_flag) {
+        volatile int never = 0;
+        for (int i = max(0, it - stages); i < it; ++i) mbar_wait(&full[i % stages], (i / stages) & 1, &never);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int it = 0; it < ng; ++it) {
+        const int s = it % stages, b = it & 1;
+        if ((it >= 2 && !mbar_wait(&pempty[b], ((it >> 1) & 1) ^ 1, abort_flag)) ||
+            !mbar_wait(&full[s], (it / stages) & 1, abort_flag)) {
+          if (!*abort_flag) atomicExch(e.err, kFp8TimeoutMma);
+          *abort_flag = 1;
+          break;
+        }
+        tc::fence_after();
+        const uint32_t w0 = smem_u32(smem + size_t(s) * K::STAGE), x0 = w0 + K::TILE_W;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_f8(tmem + b * BR, tc::desc_k(w0 + k * 32), tc::desc_k(x0 + k * 32), idesc_f8(BR), k != 0);
+        tc::commit(&empty[s]);
+        tc::commit(&pfull[b]);
+      }
+      tc::commit(done);
+      volatile int never = 0;
+      mbar_wait(done, 0, &never);
+    }
+  } else {
+    const int q = warp & 3, tid = threadIdx.x - 64;
+    // the scales of this CTA's rows and groups, while the first tiles arrive
+    for (int i = tid; i < ng * BR; i += 128) {
+      const int r = m0 + i % BR;
+      xsc[i] = r < e.m ? e.xs[(long long)r * e.groups + g0 + i / BR] : 0.f;
+    }
+    named_bar(1, 128);
+    const float* ws = e.ws + (long long)(n0 / kFp8Group) * e.wgroups + g0;
+    float w = ng > 0 ? ws[0] : 0.f;
+    for (int it = 0; it < ng; ++it) {
+      const int b = it & 1;
+      const float wn = it + 1 < ng ? ws[it + 1] : 0.f;
+      const bool ok = mbar_wait(&pfull[b], (it >> 1) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) {
+        if (lane == 0 && !*abort_flag) atomicExch(e.err, kFp8TimeoutEpi);
+        *abort_flag = 1;
+        break;
+      }
+      tc::fence_after();
+#pragma unroll
+      for (int j = 0; j < BR; j += 16) {
+        uint32_t r[16];
+        tc::tmem_ld16(tmem + (uint32_t(q * 32) << 16) + uint32_t(b * BR + j), r);
+        tc::tmem_wait_ld();
+        tc::landed(r);
+        if (j + 16 >= BR) {
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pempty[b]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const float4 x4 = *reinterpret_cast<const float4*>(xsc + it * BR + j + i);
+          acc[j + i] = fmaf(__uint_as_float(r[i]), w * x4.x, acc[j + i]);
+          acc[j + i + 1] = fmaf(__uint_as_float(r[i + 1]), w * x4.y, acc[j + i + 1]);
+          acc[j + i + 2] = fmaf(__uint_as_float(r[i + 2]), w * x4.z, acc[j + i + 2]);
+          acc[j + i + 3] = fmaf(__uint_as_float(r[i + 3]), w * x4.w, acc[j + i + 3]);
+        }
+      }
+      w = wn;
+    }
+  }
+  tc::fence_before();
+  __syncthreads();  // every MMA and load of this CTA is complete: the ring is free
+  if (warp == 1) tc::tmem_free(tmem, K::TMEM);
+  float* part = reinterpret_cast<float*>(smem);  // [row][feature]
+  if (warp >= 2) {
+    const int f = (warp & 3) * 32 + lane;
+#pragma unroll
+    for (int j = 0; j < BR; ++j) part[j * 128 + f] = acc[j];
+  }
+  cl.sync();
+  // rank r sums the rows r, r + nsplit, ... over the ranks in order
+  const int rows = min(BR, e.m - m0);
+  for (int i = threadIdx.x; i < BR * 128; i += kFewThreads) {
+    const int r = i / 128, f = i % 128, n = n0 + f;
+    if (r >= rows || r % nsplit != rank || n >= e.n) continue;
+    float v = 0.f;
+    for (int k = 0; k < nsplit; ++k) v += cl.map_shared_rank(part, k)[i];
+    if (e.bias) v += e.bias[n];
+    if (e.relu) v = v < 0.f ? 0.f : v;
+    store_as(e.y_type, e.y, size_t((long long)(m0 + r) * e.ldy + n), v);
+  }
+  cl.sync();  // peers' sums stay until everyone has read them
+}
+
+constexpr size_t kSmemMax = 227 * 1024;
+
+template <int BN>
+void launch_rows(const Fp8GemmParams& p, Args e, cudaStream_t s) {
+  using K = RowsCfg<BN>;
+  CUtensorMap tx, tw;
+  tc::make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.x, p.k, p.m, p.ldx, kKB, 128);
+  tc::make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.k, p.n, p.ldw, kKB, BN);
+  e.tiles_m = ceil_div(p.m, 128);
+  e.tiles_n = ceil_div(p.n, BN);
+  B2E_CUDA(cudaFuncSetAttribute(k_fp8_rows<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(K::SMEM)));
+  const int grid = int(std::min<long long>((long long)e.tiles_m * e.tiles_n, 148LL * K::CTAS));
+  k_fp8_rows<BN><<<grid, kThreads, K::SMEM, s>>>(tx, tw, e);
+  B2E_CUDA(cudaGetLastError());
+}
+
+template <int BR>
+void launch_few(const Fp8GemmParams& p, const Args& e, cudaStream_t s) {
+  using K = FewCfg<BR>;
+  CUtensorMap tx, tw;
+  tc::make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.x, p.k, p.m, p.ldx, kKB, BR);
+  tc::make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.k, p.n, p.ldw, kKB, 128);
+  const int tn = ceil_div(p.n, 128), tm = ceil_div(p.m, BR);
+  // as many CTAs of a cluster as fill the SMs and still have a group each
+  int split = 1;
+  while (split < 8 && split * 2 <= e.groups && (long long)tn * tm * split * 2 <= 148) split *= 2;
+  const int per = ceil_div(e.groups, split), stages = std::min(kFewStages, per);
+  const size_t smem = K::smem(stages, per);
+  B2E_CHECK(smem <= kSmemMax, kErrInvalid, "fp8_linear: k is too large");
+  B2E_CUDA(cudaFuncSetAttribute(k_fp8_few<BR>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(tn * split, tm);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {unsigned(split), 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  B2E_CUDA(cudaLaunchKernelEx(&cfg, k_fp8_few<BR>, tx, tw, e, stages));
+}
+
+}  // namespace
+
+void fp8_gemm(const Fp8GemmParams& p, cudaStream_t s) {
+  if (p.m == 0) return;
+  const int esz = int(dtype_size(p.y_type));
+  Args e{p.xs, p.ws, p.bias, p.y, p.ldy, p.m, p.n, ceil_div(p.k, kFp8Group), ceil_div(p.k, kFp8Group),
+         p.relu, p.y_type, 0, 0, 0, p.err};
+  e.vec = (reinterpret_cast<uintptr_t>(p.y) % (8 * esz)) == 0 && p.ldy % 8 == 0;
+  if (p.m <= 16) return launch_few<16>(p, e, s);
+  if (p.m <= 32) return launch_few<32>(p, e, s);
+  if (p.m <= 64) return launch_few<64>(p, e, s);
+  const long tm = ceil_div(p.m, 128);
+  // Tiles of 128 features run two CTAs an SM; tiles of 256 read less shared
+  // memory a product. The wider tile where its rounds over the SMs cost less.
+  const long r128 = (tm * ceil_div(p.n, 128) + 295) / 296, r256 = (tm * ceil_div(p.n, 256) + 147) / 148;
+  if (r256 <= r128)
+    launch_rows<256>(p, e, s);
+  else
+    launch_rows<128>(p, e, s);
+}
+
+namespace tc {
+
+void make_map(CUtensorMap* m, CUtensorMapDataType type, int size, const void* base, uint64_t inner, uint64_t rows,
+              uint64_t ld, uint32_t box_inner, uint32_t box_rows) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  B2E_CHECK(fn != nullptr, kErrCuda, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[2] = {inner, rows};
+  const cuuint64_t strides[1] = {ld * uint64_t(size)};
+  const cuuint32_t box[2] = {box_inner, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  B2E_CHECK(r == CUDA_SUCCESS, kErrCuda, "cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+}
+
+}  // namespace tc
+}  // namespace b2e

@@ -9,11 +9,18 @@ views (they are made contiguous); the state may not, because it is written in
 place. Errors raise AssertionError, like the reference's wrappers
 (model/kernels.py:85-122). The computation is libb2e.so's CUDA kernels on the
 current torch stream; there is no CPU path.
+
+Beside them, the operators of a Mamba2 layer over a whole run of tokens (a
+symbol's history in one call instead of one call a token), which the reference
+does not have: ``rms_norm_fp8``, ``fp8_linear`` with its quantisers,
+``causal_conv`` and ``mamba2_scan``, the last two over the packed sequences of a
+``SequenceBatch``. They serve: nothing here has a gradient.
 """
 
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
@@ -144,3 +151,323 @@ def cast_linear(x, weight, bias=None, relu: bool = False, err=None):
     _lib.check(_lib.lib().b2e_linear(_ptr(x), _TORCH_DTYPES[x.dtype], x.shape[0], x.shape[1], _ptr(weight), wt,
                                      _ptr(bias), weight.shape[0], int(relu), _ptr(y), _ptr(err), _stream(x.device)))
     return y
+
+
+# ------------------------------------------------------------ runs of tokens
+
+FP8_GROUP = 128  # columns of a row (rows and columns of a weight's block) that share a scale
+
+
+class SequenceBatch:
+    """Plan of a packed batch of sequences, kept for every call on that batch.
+
+    Sequence i has ``lengths[i]`` tokens (zero: its state stays as it is), packed
+    one after the other in the operands' rows, and lives in row ``slots[i]`` of the
+    state tables (default: row i). Everything is checked here, on the host: lengths
+    are not negative, slots distinct and inside the ``state_rows`` rows of the
+    smallest table the plan is used with (default: up to the highest slot). The
+    plan's device arrays belong to ``device``; keep the plan until the work that
+    uses it is done.
+    """
+
+    def __init__(self, lengths: Sequence[int], slots: Optional[Sequence[int]] = None, *,
+                 state_rows: Optional[int] = None, device=None):
+        lengths = [int(n) for n in lengths]
+        assert all(n >= 0 for n in lengths), "lengths must not be negative"
+        self.tokens = sum(lengths)
+        assert self.tokens < 2 ** 31 and len(lengths) < 2 ** 31, "a batch has less than 2^31 tokens"
+        if slots is not None:
+            slots = [int(s) for s in slots]
+            assert len(slots) == len(lengths), f"{len(slots)} slots for {len(lengths)} sequences"
+            assert len(set(slots)) == len(slots), "slots must be distinct"
+            assert all(s >= 0 for s in slots), "slots must not be negative"
+        need = (max(slots) + 1 if slots else 0) if slots is not None else len(lengths)
+        self.state_rows = need if state_rows is None else int(state_rows)
+        assert need <= self.state_rows < 2 ** 31, f"slots reach row {need - 1} of {self.state_rows} state rows"
+        self.lengths = tuple(lengths)
+        self.slots = tuple(range(len(lengths))) if slots is None else tuple(slots)
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        single = all(n == 1 for n in lengths)  # one token a sequence: the step kernels, which need no starts
+        starts = [0]
+        for n in lengths:
+            starts.append(starts[-1] + n)
+        host = ([] if single else starts) + ([] if slots is None else slots)
+        self._arrays = torch.tensor(host, dtype=torch.int32).to(self.device)
+        at = self._arrays.data_ptr()
+        self._c = _lib.SequencesC(None if single else at, None if slots is None else at + (0 if single else 4 * len(starts)),
+                                  len(lengths), self.tokens, self.state_rows, max(lengths, default=0))
+
+    def __len__(self) -> int:
+        return len(self.lengths)
+
+
+class NormFp8(NamedTuple):
+    """``rms_norm_fp8``'s results: e4m3 values, their scales (rows, groups of 128
+    columns), the sum with the residual and the normed row (None where not asked)."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+    total: Optional[torch.Tensor]
+    normed: Optional[torch.Tensor]
+
+
+def _call(name: str, device, *args) -> None:
+    """One C-ABI call on `device`'s current stream."""
+    fn = getattr(_lib.lib(), name)
+    if torch.cuda.current_device() == device.index:
+        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
+def _at(t) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t: torch.Tensor):
+    """A 2-D operand whose rows are contiguous (copied if they are not) and its row stride."""
+    n, c = t.shape
+    if (c > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < c):
+        t = t.contiguous()
+    return t, (t.stride(0) if n > 1 else c)
+
+
+def _rows8(t: torch.Tensor):
+    """The same for e4m3 rows, which start on 16-byte boundaries."""
+    n, k = t.shape
+    if (k > 1 and t.stride(1) != 1) or t.data_ptr() % 16 or (n > 1 and (t.stride(0) < k or t.stride(0) % 16)):
+        wide = torch.empty(n, -(-k // 16) * 16, dtype=t.dtype, device=t.device)
+        wide[:, :k].copy_(t)
+        t = wide[:, :k]
+    return t, (t.stride(0) if n > 1 else -(-k // 16) * 16)
+
+
+def _empty8(rows: int, cols: int, device):
+    """Empty e4m3 rows, padded so that each starts on a 16-byte boundary, and scales' columns."""
+    wide = torch.empty(rows, -(-cols // 16) * 16, dtype=torch.float8_e4m3fn, device=device)
+    return wide[:, :cols] if cols % 16 else wide, -(-cols // FP8_GROUP)
+
+
+def _float(t: torch.Tensor, name: str) -> int:
+    assert t.dtype in _TORCH_DTYPES, f"{name} must be float32, bfloat16 or float16, got {t.dtype}"
+    return _TORCH_DTYPES[t.dtype]
+
+
+def _vector(t, n: int, name: str, device):
+    """An optional float32 vector of n values."""
+    if t is None:
+        return None
+    assert t.dtype == torch.float32 and tuple(t.shape) == (n,), f"{name} must be float32 ({n},), got {t.dtype} {tuple(t.shape)}"
+    assert t.device == device, f"{name} must be on {device}, it is on {t.device}"
+    return t.contiguous()
+
+
+def _on_gpu(t: torch.Tensor, name: str) -> None:
+    assert t.is_cuda, f"{name} must be a CUDA tensor (there is no CPU path)"
+
+
+def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-5, keep_norm: bool = False) -> NormFp8:
+    """RMS norm of ``x + residual`` (rows, cols) with an 8-bit output for ``fp8_linear``.
+
+    v = x + residual; n = v / sqrt(mean(v^2) + eps) * weight, all in float32; each 128
+    columns of a row get scale = max(max|n| / 448, 2^-100) and q = e4m3(n / scale).
+    ``total`` is v in the residual's type (x's or float32), the next layer's residual;
+    ``keep_norm`` adds n in x's type, for the projections that stay in float32. A NaN or
+    an infinity makes its whole row NaN, as the formula does.
+    """
+    assert x.dim() == 2 and x.shape[1] > 0, f"x must be (rows, cols), got {tuple(x.shape)}"
+    xt = _float(x, "x")
+    rows, cols = x.shape
+    rt, ldr = xt, 0
+    if residual is not None:
+        assert residual.shape == x.shape, f"residual must be {tuple(x.shape)}, got {tuple(residual.shape)}"
+        assert residual.dtype in (x.dtype, torch.float32), f"residual must be {x.dtype} or float32, got {residual.dtype}"
+        assert residual.device == x.device, f"residual must be on {x.device}, it is on {residual.device}"
+        rt = _TORCH_DTYPES[residual.dtype]
+        residual, ldr = _rows(residual)
+    weight = _vector(weight, cols, "weight", x.device)
+    _on_gpu(x, "x")
+    x, ldx = _rows(x)
+    q, groups = _empty8(rows, cols, x.device)
+    scale = torch.empty(rows, groups, dtype=torch.float32, device=x.device)
+    total = None if residual is None else torch.empty(rows, cols, dtype=residual.dtype, device=x.device)
+    normed = torch.empty(rows, cols, dtype=x.dtype, device=x.device) if keep_norm else None
+    if rows:
+        _call("b2e_rms_norm_fp8", x.device, _at(x), xt, ldx, _at(residual), rt, ldr, _at(weight), eps, rows, cols, _at(q),
+              -(-cols // 16) * 16, _at(scale), _at(total), _at(normed))
+    return NormFp8(q, scale, total, normed)
+
+
+def quantize_fp8(x):
+    """e4m3 values of x (rows, cols) and the scale of each 128 columns of a row, (rows, ceil(cols / 128))."""
+    assert x.dim() == 2 and x.shape[1] > 0, f"x must be (rows, cols), got {tuple(x.shape)}"
+    xt = _float(x, "x")
+    _on_gpu(x, "x")
+    x, ldx = _rows(x)
+    rows, cols = x.shape
+    q, groups = _empty8(rows, cols, x.device)
+    scale = torch.empty(rows, groups, dtype=torch.float32, device=x.device)
+    if rows:
+        _call("b2e_quantize_fp8", x.device, _at(x), xt, ldx, rows, cols, _at(q), -(-cols // 16) * 16, _at(scale))
+    return q, scale
+
+
+def quantize_fp8_weight(weight):
+    """e4m3 values of a weight (out, in) and the scale of each 128 x 128 block, (ceil(out / 128), ceil(in / 128))."""
+    assert weight.dim() == 2 and weight.numel() > 0, f"weight must be (out, in), got {tuple(weight.shape)}"
+    wt = _float(weight, "weight")
+    _on_gpu(weight, "weight")
+    weight, ldw = _rows(weight)
+    rows, cols = weight.shape
+    q, groups = _empty8(rows, cols, weight.device)
+    scale = torch.empty(-(-rows // FP8_GROUP), groups, dtype=torch.float32, device=weight.device)
+    _call("b2e_quantize_fp8_weight", weight.device, _at(weight), wt, ldw, rows, cols, _at(q), -(-cols // 16) * 16, _at(scale))
+    return q, scale
+
+
+def fp8_linear(q, scale, wq, wscale, bias=None, relu: bool = False, out_dtype=torch.float32):
+    """The projection of 8-bit rows by an 8-bit weight, beside ``cast_linear``.
+
+    ``q`` (m, k) with ``scale`` (m, ceil(k / 128)) from ``rms_norm_fp8`` or
+    ``quantize_fp8``; ``wq`` (n, k) with ``wscale`` (ceil(n / 128), ceil(k / 128)) from
+    ``quantize_fp8_weight``; ``bias`` float32 (n,). Each group's 128 products are summed
+    and the groups' sums scaled and added in float32; the result is rounded once to
+    ``out_dtype``. Operands whose rows do not start on 16-byte boundaries are copied.
+    """
+    assert q.dim() == 2 and wq.dim() == 2 and q.shape[1] == wq.shape[1] and wq.numel() > 0, \
+        f"q (m, k) and wq (n, k) expected, got {tuple(q.shape)} and {tuple(wq.shape)}"
+    assert q.dtype == wq.dtype == torch.float8_e4m3fn, f"q and wq must be float8_e4m3fn, got {q.dtype} and {wq.dtype}"
+    m, k = q.shape
+    n, g = wq.shape[0], -(-k // FP8_GROUP)
+    dev = q.device
+    for t, shape, name in ((scale, (m, g), "scale"), (wscale, (-(-n // FP8_GROUP), g), "wscale")):
+        assert t.dtype == torch.float32 and tuple(t.shape) == shape, f"{name} must be float32 {shape}, got {t.dtype} {tuple(t.shape)}"
+        assert t.device == dev, f"{name} must be on {dev}, it is on {t.device}"
+    assert wq.device == dev, f"wq must be on {dev}, it is on {wq.device}"
+    assert out_dtype in _TORCH_DTYPES, f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}"
+    bias = _vector(bias, n, "bias", dev)
+    _on_gpu(q, "q")
+    y = torch.empty(m, n, dtype=out_dtype, device=dev)
+    if m:
+        q, ldq = _rows8(q)
+        wq, ldw = _rows8(wq)
+        scale, wscale = scale.contiguous(), wscale.contiguous()
+        _call("b2e_fp8_linear", dev, _at(q), ldq, _at(scale), m, k, _at(wq), ldw, _at(wscale), n, _at(bias), int(relu), _at(y),
+              _TORCH_DTYPES[out_dtype], n)
+    return y
+
+
+def _plan(seqs: Optional[SequenceBatch], rows: int, table: torch.Tensor, name: str):
+    """(C plan, tokens) of a call over `rows` operand rows and a state table."""
+    if seqs is None:
+        assert rows == table.shape[0], f"without a SequenceBatch every row of {name} steps: {rows} rows for {table.shape[0]}"
+        return None, rows
+    assert seqs.tokens <= rows, f"the batch has {seqs.tokens} tokens, the operands {rows} rows"
+    assert seqs.state_rows <= table.shape[0], f"the batch's slots need {seqs.state_rows} state rows, {name} has {table.shape[0]}"
+    assert seqs.device == table.device, f"the batch is on {seqs.device}, {name} on {table.device}"
+    return C.byref(seqs._c), seqs.tokens
+
+
+def _out(like, rows: int, tokens: int):
+    """An output of the operands' shape; rows of no sequence are zero."""
+    y = torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if rows > tokens:
+        y[tokens:].zero_()
+    return y
+
+
+def causal_conv(window, x, weight, bias=None, seqs: Optional[SequenceBatch] = None, silu: bool = False):
+    """CausalConv1d (model/modules.py:37-41) over every token of packed sequences.
+
+    ``window`` (state rows, channels, taps - 1) float32 holds each sequence's last inputs
+    and is updated IN PLACE (rows of no sequence, and of empty ones, stay bit for bit);
+    ``x`` (rows, channels); ``weight`` (channels, taps), 2 to 4 taps, and ``bias`` float32.
+    y[t] = sum_j weight[j] v[t + j] + bias over v = window ++ sequence, with SiLU if asked,
+    rounded once to x's type. Without ``seqs`` each row of x is one token of that row of
+    ``window``. Rows of x behind the batch's tokens are not read and give zeros.
+    """
+    assert window.dim() == 3 and 1 <= window.shape[2] <= 3, f"window must be (rows, channels, 1..3), got {tuple(window.shape)}"
+    assert window.dtype == torch.float32, f"window must be fp32, got {window.dtype}"
+    assert window.is_contiguous(), "window must be contiguous, it is written in place"
+    ch, taps, dev = window.shape[1], window.shape[2] + 1, window.device
+    assert ch > 0 and x.dim() == 2 and x.shape[1] == ch, f"x must be (rows, {ch}), got {tuple(x.shape)}"
+    xt = _float(x, "x")
+    assert x.device == dev, f"x must be on {dev}, it is on {x.device}"
+    assert weight.dtype == torch.float32 and tuple(weight.shape) == (ch, taps), \
+        f"weight must be float32 {(ch, taps)}, got {weight.dtype} {tuple(weight.shape)}"
+    assert weight.device == dev, f"weight must be on {dev}, it is on {weight.device}"
+    bias = _vector(bias, ch, "bias", dev)
+    rows = x.shape[0]
+    plan, tokens = _plan(seqs, rows, window, "window")
+    _on_gpu(window, "window")
+    y = _out(x, rows, tokens)
+    if tokens:
+        x, ldx = _rows(x)
+        weight = weight.contiguous()
+        _call("b2e_causal_conv", dev, plan, _at(window), _at(x), xt, ldx, rows, ch, _at(weight), _at(bias), taps, int(silu),
+              _at(y), ch)
+    return y
+
+
+def mamba2_scan(ssm, x, b, c, dt, a, seqs: Optional[SequenceBatch] = None, d=None, z=None, softplus: bool = True):
+    """Mamba2's recurrence (model/mamba2.py:128-165) over every token of packed sequences.
+
+    t = softplus(dt) (dt itself without ``softplus``); ssm <- exp(a t) ssm + t (b outer x);
+    y = (sum_c c * ssm + d x) * silu(z). ``ssm`` (state rows, heads, size, state) float32 is
+    updated IN PLACE; rows of no sequence, and of empty ones, stay bit for bit. ``x``, ``z``
+    (rows, heads, size), ``b``, ``c`` (rows, state), state up to 256, all of one type; ``dt``
+    (rows, heads), ``a`` and ``d`` (heads,) float32. The state and all sums are float32 and y
+    is rounded once to x's type. Without ``seqs`` each row is one token of that row of
+    ``ssm``, as in ``mamba2_step``. Rows behind the batch's tokens are not read and give zeros.
+    """
+    _scan_state_ok(ssm)
+    nrows, h, p, n = ssm.shape
+    dev = ssm.device
+    assert x.dim() == 3 and tuple(x.shape[1:]) == (h, p), f"x must be (rows, {h}, {p}), got {tuple(x.shape)}"
+    xt = _float(x, "x")
+    rows = x.shape[0]
+    for t, shape, name in ((x, (rows, h, p), "x"), (z, (rows, h, p), "z"), (b, (rows, n), "b"), (c, (rows, n), "c")):
+        if t is not None:
+            assert t.dtype == x.dtype and tuple(t.shape) == shape, f"{name} must be {x.dtype} {shape}, got {t.dtype} {tuple(t.shape)}"
+            assert t.device == dev, f"{name} must be on {dev}, it is on {t.device}"
+    assert dt.dtype == torch.float32 and tuple(dt.shape) == (rows, h), f"dt must be float32 {(rows, h)}, got {dt.dtype} {tuple(dt.shape)}"
+    assert dt.device == dev, f"dt must be on {dev}, it is on {dt.device}"
+    assert a is not None, "a must be given"
+    a, d = _vector(a, h, "a", dev), _vector(d, h, "d", dev)
+    plan, tokens = _plan(seqs, rows, ssm, "ssm")
+    _on_gpu(ssm, "ssm")
+    y = _out(x, rows, tokens)
+    if tokens:
+        x, ldx = _rows(x.reshape(rows, h * p))
+        z, ldz = (None, 0) if z is None else _rows(z.reshape(rows, h * p))
+        (b, ldb), (c, ldc), (dt, lddt) = _rows(b), _rows(c), _rows(dt)
+        args = _lib.ScanArgsC(ssm.data_ptr(), x.data_ptr(), b.data_ptr(), c.data_ptr(), dt.data_ptr(), a.data_ptr(), _at(d),
+                              _at(z), y.data_ptr(), ldx, ldb, ldc, lddt, ldz, h * p, rows, h, p, n, xt, int(softplus))
+        ref, work, size = C.byref(args), None, 0
+        if seqs is not None:
+            need = C.c_int64()
+            _lib.check(_lib.lib().b2e_mamba2_scan_workspace(plan, ref, C.byref(need)))
+            size = need.value
+            work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        _call("b2e_mamba2_scan", dev, plan, ref, _at(work), size)
+    return y
+
+
+def _scan_state_ok(ssm: torch.Tensor) -> None:
+    assert ssm.dtype == torch.float32, f"ssm must be fp32, got {ssm.dtype}"
+    assert ssm.dim() == 4 and min(ssm.shape[1:]) > 0, f"ssm must be (rows, heads, size, state), got {tuple(ssm.shape)}"
+    assert ssm.is_contiguous(), "ssm must be contiguous, it is written in place"
+    assert ssm.shape[3] <= 256, f"a state has at most 256 columns, got {ssm.shape[3]}"
+    assert ssm.shape[0] == 0 or not ssm.is_cuda or ssm.data_ptr() % 16 == 0 or ssm.shape[3] % 4, "ssm must start on a 16-byte boundary"
+
+
+def device_error(device=None) -> int:
+    """Error word of this module's run-of-tokens operators on a device (b2e_seqops_device_error):
+    0, or the code of a bounded wait that ran out. Waits for the device, reads and clears it."""
+    code = C.c_int32()
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().b2e_seqops_device_error(C.byref(code)))
+    return code.value

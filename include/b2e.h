@@ -221,6 +221,91 @@ B2E_API int b2e_linear_static(const void* x, int32_t x_dtype, int32_t m, int32_t
                               int32_t w_dtype, const void* bias, int32_t n, int32_t act, float* y,
                               int32_t* h_err, void* stream);
 
+/* ---- runs of tokens: the Mamba2 layer's operators over packed sequences ----
+ * No counterpart in the reference, which steps one token at a time: these take a
+ * symbol's whole run of tokens in one call and leave its state where as many
+ * single steps would. Device pointers; row strides (ld*) in elements; sums,
+ * statistics, scales and states are float32; dtype is B2E_DTYPE_* of the
+ * activations. A call works on the current device and allocates nothing.
+ *
+ * Plan of a packed batch: sequence i is rows [starts[i], starts[i + 1]) of the
+ * operands (starts[0] = 0, starts[seqs] = tokens) and row slots[i] of the state
+ * table (slots distinct; two sequences in one state row race). starts NULL: one
+ * token a sequence; slots NULL: state row i. longest: tokens of the longest
+ * sequence; the kernels are chosen by it. A null plan is one token a sequence
+ * and state row i for every row of the operands. Rows of the operands behind
+ * `tokens` are not read, and their outputs not written. A plan whose device
+ * arrays leave the operands or the table steps no row of the sequence in
+ * question and sets the error word. */
+typedef struct b2e_sequences {
+  const int32_t* starts; /* [seqs + 1] */
+  const int32_t* slots;  /* [seqs] */
+  int32_t seqs;
+  int32_t tokens;
+  int32_t state_rows;
+  int32_t longest;
+} b2e_sequences;
+
+/* Error word of these operators on the current device: 0, or the code of a
+ * bounded wait that ran out (the call's output is not valid) or 1 for a plan out
+ * of range. Waits for the device, reads and clears it. */
+B2E_API int b2e_seqops_device_error(int32_t* code);
+
+/* v = x + residual; n = v / sqrt(mean(v^2) + eps) * weight; for each 128 columns
+ * scale = max(max|n| / 448, 2^-100) and q = e4m3(n / scale). residual NULL: v = x
+ * (and total NULL); weight NULL: ones. total (residual's dtype) receives v, normed
+ * (x's dtype, may be NULL) n, both with rows of cols values. r_dtype is x_dtype or
+ * float32. scale is [rows, ceil(cols / 128)]. */
+B2E_API int b2e_rms_norm_fp8(const void* x, int32_t x_dtype, int64_t ldx, const void* residual, int32_t r_dtype, int64_t ldr,
+                     const float* weight, float eps, int32_t rows, int32_t cols, void* q, int64_t ldq, float* scale,
+                     void* total, void* normed, void* stream);
+/* q and scale of x itself, without the norm. */
+B2E_API int b2e_quantize_fp8(const void* x, int32_t x_dtype, int64_t ldx, int32_t rows, int32_t cols, void* q, int64_t ldq,
+                     float* scale, void* stream);
+/* A weight in e4m3 with a scale for each block of 128 rows and 128 columns:
+ * scale is [ceil(rows / 128), ceil(cols / 128)]. */
+B2E_API int b2e_quantize_fp8_weight(const void* w, int32_t w_dtype, int64_t ldw, int32_t rows, int32_t cols, void* q,
+                     int64_t ldq, float* scale, void* stream);
+/* y[m, n] = act(sum_g scale[m, g] wscale[n / 128, g] sum_{k in g} q[m, k] wq[n, k] + bias[n]),
+ * groups g of 128 columns, rounded once to y_dtype; act 0 = none, 1 = ReLU. Rows
+ * of q and wq start on 16-byte boundaries (a stride padded to 16). */
+B2E_API int b2e_fp8_linear(const void* q, int64_t ldq, const float* scale, int32_t m, int32_t k, const void* wq, int64_t ldw,
+                   const float* wscale, int32_t n, const float* bias, int32_t act, void* y, int32_t y_dtype, int64_t ldy,
+                   void* stream);
+/* CausalConv1d (model/modules.py:37-41) over every token: window is
+ * [state_rows, channels, taps - 1] float32, weight [channels, taps], taps 2 to 4;
+ * act 0 = none, 1 = SiLU. y may not overlap x. */
+B2E_API int b2e_causal_conv(const b2e_sequences* plan, float* window, const void* x, int32_t dtype, int64_t ldx, int32_t rows,
+                    int32_t channels, const float* weight, const float* bias, int32_t taps, int32_t act, void* y,
+                    int64_t ldy, void* stream);
+/* Mamba2's recurrence (model/mamba2.py:128-165) over every token:
+ *   t = softplus(dt) (dt itself when softplus is 0); h <- exp(a t) h + t x b^T;
+ *   y = (h c + d x) * silu(z)
+ * ssm is [state_rows, heads, size, state] float32, updated in place; x, z and y
+ * have rows of heads * size values, b and c of state (1..256), dt of heads
+ * float32; d and z may be NULL. Long sequences in a small batch are split over
+ * the device, which takes b2e_mamba2_scan_workspace() bytes (16-byte aligned, 0
+ * and NULL where none is needed; the size depends on the plan and the sizes
+ * alone). y may not overlap an input. */
+typedef struct b2e_scan_args {
+  float* ssm;
+  const void* x;
+  const void* b;
+  const void* c;
+  const float* dt;
+  const float* a;
+  const float* d;
+  const void* z;
+  void* y;
+  int64_t ldx, ldb, ldc, lddt, ldz, ldy;
+  int32_t rows; /* of the operands */
+  int32_t heads, size, state;
+  int32_t dtype;
+  int32_t softplus;
+} b2e_scan_args;
+B2E_API int b2e_mamba2_scan_workspace(const b2e_sequences* plan, const b2e_scan_args* args, int64_t* bytes);
+B2E_API int b2e_mamba2_scan(const b2e_sequences* plan, const b2e_scan_args* args, void* work, int64_t work_bytes, void* stream);
+
 /* ---- one recurrent layer with its own state table ----
  * Weights are keyed like that layer's own state_dict() (no prefix). */
 B2E_API int b2e_layer_create(int32_t kind, const b2e_model_config* cfg, const b2e_engine_options* opt,
