@@ -359,6 +359,7 @@ template <int T>
 void launch_type(const ScanParams& p, cudaStream_t s) {
   if (single_tokens(p)) return launch_step<T>(p, s);
   const int seg = scan_segment(p);
+  if (scan_tc_eligible(p)) return scan_tc(p, seg, s);
   ScanWork wk{};
   if (seg > 0) {
     wk = scan_work(p, seg);
@@ -387,10 +388,11 @@ ScanWork scan_work(const ScanParams& p, int seg) {
 // Splitting a sequence costs a second pass over its tokens (the contributions)
 // and its segments' states in the workspace, so it is done only where whole
 // sequences would leave SMs idle: segments of a multiple of 128 tokens, as many
-// as give each SM four CTAs.
+// as give each SM four CTAs of the recurrence kernel, or one of the chunked one.
 int scan_segment(const ScanParams& p) {
   if (single_tokens(p)) return 0;
-  const long long per = (long long)p.heads * ceil_div(p.size, 64), want = 148 * 4;
+  const bool tc = scan_tc_eligible(p);
+  const long long per = tc ? (p.heads + 1) / 2 : (long long)p.heads * ceil_div(p.size, 64), want = tc ? 148 : 148 * 4;
   if (p.plan.seqs * per >= want || p.plan.longest <= 256) return 0;
   const long long segs = std::max<long long>(1, want / per);
   const long long len = (p.plan.tokens + segs - 1) / segs;

@@ -11,6 +11,10 @@ struct ScanWork {
   float* state = nullptr;      // [segments, heads, size, state]
 };
 ScanWork scan_work(const ScanParams& p, int seg);
+// The chunked tensor-core kernel (scan_tc.cu): whether it takes these operands,
+// and the scan itself.
+bool scan_tc_eligible(const ScanParams& p);
+void scan_tc(const ScanParams& p, int seg, cudaStream_t s);
 void scan_join(const ScanParams& p, const ScanWork& wk, int seg, cudaStream_t s);
 
 }  // namespace b2e
