@@ -46,12 +46,15 @@ namespace {
 constexpr int Q = 128;                       // tokens of a chunk
 constexpr uint32_t kTile = Q * 128;          // 128 rows of 128 bytes
 constexpr int kXSlots = 3;
-constexpr int kTcThreads = 512;
+constexpr int kTcThreads = 896;
+constexpr int kVecs = 3;                     // chunks whose decays are held
 enum ScanError : int { kScanTimeout = 131 };
 
-// TMEM columns (of 512): G, and S of the second head in its place; S of the
-// first; two buffers of the state's operand; Y and H of both heads.
-constexpr uint32_t cG = 0, cS1 = 0, cS0 = 128, cXW = 192, cY = 256, cH = 384;
+// TMEM columns (of 512): G, and S of both heads in its place (each 16 columns of
+// G become 8 of either head's S in bf16 pairs); the buffers of the state's
+// operand; Y and H of both heads.
+constexpr uint32_t cG = 0, cXW = 128, cY = 256, cH = 384;
+__device__ __forceinline__ uint32_t s_col(int h, int k) { return cG + k * 16 + h * 8; }  // tokens 16 k..
 
 // kind::f16, bf16 x bf16, float32 accumulator, M = 128.
 __host__ __device__ constexpr uint32_t idesc_bf16(int n, bool b_mn) {
@@ -90,6 +93,42 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// Two float32 lanes in one instruction, each rounded as the scalar one.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2(uint32_t a, uint32_t b) { return f2(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ void split(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(F2 a) {
+  float x, y;
+  split(a, x, y);
+  return pack_bf16(x, y);
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
@@ -111,13 +150,14 @@ __device__ __forceinline__ Pair shfl(Pair a, int src) {
   return {__shfl_sync(0xffffffffu, a.hi, src), __shfl_sync(0xffffffffu, a.lo, src)};
 }
 
-// Decays of one head and chunk, exponents in powers of two.
+// Decays of one head and chunk; c in powers of two.
 struct Vec {
-  float4 tok[Q];    // c[s] (hi, lo), dt[s], exp(c[T] - c[s]) dt[s]
-  float start[Q];   // exp(c[t])
-  float row[Q];     // exp(c[t] - c[first token of its 32-block, exclusive])
-  float col[192];   // exp(c[before block i] - c[s]) dt[s] for s before block i: 32 values for i = 1, 64, 96
-  float total;      // exp(c[T])
+  float neg[Q];   // -(c[s] - base[s / 32])
+  float dt[Q];
+  float w[Q];     // exp(c[T] - c[s]) dt[s]
+  float col[192]; // exp(base[i] - c[s]) dt[s] for s before block i: 32 values for i = 1, 64, 96
+  float base[4];  // c before each block of 32 tokens
+  float total;    // exp(c[T])
   float pad[3];
 };
 
@@ -126,8 +166,8 @@ struct TcCfg {
   static constexpr uint32_t CB = NB * kTile;  // bytes of a chunk of C (or B)
   static constexpr uint32_t oC = 0, oB = CB, STAGE = 2 * CB;
   static constexpr uint32_t oX = 2 * STAGE, oH = oX + kXSlots * kTile, oV = oH + NB * kTile;
-  static constexpr uint32_t oBad = oV + 4 * sizeof(Vec);            // [2][128] first token that is not finite, [2][4] flags
-  static constexpr uint32_t oBar = oBad + 2 * 128 * 4 + 2 * 4 * 4;
+  static constexpr uint32_t oBad = oV + kVecs * 2 * sizeof(Vec);    // [kVecs][2][128] first token that is not finite, [kVecs][8] flags
+  static constexpr uint32_t oBar = oBad + kVecs * (2 * 128 + 8 * 4);
   static constexpr size_t SMEM = oBar + 512 + 1024;
 };
 
@@ -168,39 +208,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
-  Vec* vec = reinterpret_cast<Vec*>(smem + K::oV);  // [chunk parity][head]
-  int* bad = reinterpret_cast<int*>(smem + K::oBad);
-  int* anybad = bad + 2 * 128;
+  Vec* vec = reinterpret_cast<Vec*>(smem + K::oV);  // [chunk % kVecs][head]
+  uint8_t* bad = smem + K::oBad;
+  int* anybad = reinterpret_cast<int*>(bad + kVecs * 2 * 128);
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + K::oBar);
-  uint64_t *cbfull = bar, *cbempty = bar + 2, *xfull = bar + 4, *xempty = bar + 7, *vfull = bar + 10, *vempty = bar + 12,
-           *gfull = bar + 14, *sfull = bar + 15, *y2full = bar + 17, *y2scaled = bar + 18, *yfull = bar + 19, *yfree = bar + 20,
-           *hready = bar + 21, *hdone = bar + 22, *xwfull = bar + 23, *xwempty = bar + 25, *xscan = bar + 27, *done = bar + 29;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 30);
+  uint64_t *cbfull = bar, *cbempty = bar + 2, *xfull = bar + 4, *xempty = bar + 7, *vfull = bar + 10, *vempty = bar + 13,
+           *xwfull = bar + 16, *xwempty = bar + 18, *xscan = bar + 20, *gfull = bar + 23, *sfull = bar + 24, *y2full = bar + 25,
+           *y2scaled = bar + 26, *yfull = bar + 27, *yfree = bar + 28, *hready = bar + 29, *hdone = bar + 30, *done = bar + 31;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&cbfull[i], 1);
-      mbar_init(&cbempty[i], 1);
-      mbar_init(&vfull[i], 2);
-      mbar_init(&vempty[i], ENDS ? 4 : 12);
-      mbar_init(&sfull[i], 4);
+      mbar_init(&cbempty[i], ENDS ? 1 : 2);
       mbar_init(&xwfull[i], 4);
       mbar_init(&xwempty[i], 1);
-      mbar_init(&xscan[i], 4);
+    }
+    for (int i = 0; i < kVecs; ++i) {
+      mbar_init(&vfull[i], 1);
+      mbar_init(&vempty[i], ENDS ? 8 : 24);
+      mbar_init(&xscan[i], 8);
     }
     for (int i = 0; i < kXSlots; ++i) {
       mbar_init(&xfull[i], 1);
-      mbar_init(&xempty[i], ENDS ? 2 : 7);  // two warps of the state's, S X, four warps of y's
+      mbar_init(&xempty[i], ENDS ? 4 : 9);  // four warps of the state's, S X, four warps of y's
     }
     mbar_init(gfull, 1);
+    mbar_init(sfull, 8);
     mbar_init(y2full, 1);
-    mbar_init(y2scaled, 4);
+    mbar_init(y2scaled, 8);
     mbar_init(yfull, 1);
-    mbar_init(yfree, 4);
-    mbar_init(hready, 4);
+    mbar_init(yfree, 8);
+    mbar_init(hready, 8);
     mbar_init(hdone, 1);
-    mbar_init(done, 1);
+    mbar_init(done, ENDS ? 1 : 2);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
@@ -215,16 +257,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;  // this warp's TMEM lanes
 
-  // Every thread of a warp waits; false (for all of them) once a wait anywhere ran out.
-  auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
-    const bool ok = mbar_wait(b, parity, abort_flag);
-    if (__all_sync(0xffffffffu, ok)) return true;
-    if (lane == 0) {
-      if (!*abort_flag) atomicExch(p.err, kScanTimeout);
-      *abort_flag = 1;
-    }
-    return false;
+  // The roles' code runs beside one another out of one instruction cache, so it is
+  // kept short: loops stay rolled and a wait is a handful of instructions. A wait
+  // is bounded by its polls (a poll suspends the thread for a while; 2^22 are from
+  // a tenth of a second to seconds), and its role winds down when they run out.
+  auto poll = [&](uint64_t* b, uint32_t parity) -> bool {
+    int n = 0;
+    while (!mbar_try(b, parity))
+      if (++n == 1 << 22) return false;
+    return true;
   };
+  auto failed = [&] {
+    atomicExch(p.err, kScanTimeout);
+    *abort_flag = 1;
+  };
+  // Every thread of a warp waits, with one answer for all of them.
+  auto wait = [&](uint64_t* b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, poll(b, parity)); };
   auto arrive = [&](uint64_t* b) {
     __syncwarp();
     if (lane == 0) mbar_arrive(b);
@@ -234,238 +282,291 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ---- loads
     if (lane == 0) {
       int c = 0, u = 0;
-      auto wait1 = [&](uint64_t* b, uint32_t parity) {
-        if (mbar_wait(b, parity, abort_flag)) return true;
-        if (!*abort_flag) atomicExch(p.err, kScanTimeout);
-        *abort_flag = 1;
-        return false;
-      };
-      for (; c < chunks; ++c) {
+      bool ok = true;
+#pragma unroll 1
+      for (; c < chunks && ok; ++c) {
         const int st = c & 1, row = t.first + c * Q;
-        if (c >= 2 && !wait1(&cbempty[st], ((c >> 1) & 1) ^ 1)) break;
+        if (c >= 2 && !(ok = poll(&cbempty[st], ((c >> 1) & 1) ^ 1))) break;
         uint8_t* s = smem + st * K::STAGE;
         mbar_expect_tx(&cbfull[st], (ENDS ? 1 : 2) * K::CB);
+#pragma unroll 1
         for (int i = 0; i < NB; ++i) {
           tc::tma_load_2d(s + K::oB + i * kTile, &mb, i * 64, row, &cbfull[st]);
           if (!ENDS) tc::tma_load_2d(s + K::oC + i * kTile, &mc, i * 64, row, &cbfull[st]);
         }
+#pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           const int sl = u % kXSlots;
-          if (u >= kXSlots && !wait1(&xempty[sl], ((u / kXSlots) & 1) ^ 1)) break;
+          if (u >= kXSlots && !(ok = poll(&xempty[sl], ((u / kXSlots) & 1) ^ 1))) break;
           mbar_expect_tx(&xfull[sl], kTile);
           tc::tma_load_2d(smem + K::oX + sl * kTile, &mx, (h0 + h) * 64, row, &xfull[sl]);
           ++u;
         }
-        if (*abort_flag) {
-          ++c;
-          break;
-        }
       }
-      if (*abort_flag) {  // every load issued lands before the CTA leaves (bounded)
-        volatile int never = 0;
-        for (int i = max(0, c - 2); i < c; ++i) mbar_wait(&cbfull[i & 1], (i >> 1) & 1, &never);
-        for (int i = max(0, u - kXSlots); i < u; ++i) mbar_wait(&xfull[i % kXSlots], (i / kXSlots) & 1, &never);
+      if (!ok) {
+        failed();
+        // every load issued lands before the CTA leaves (bounded)
+        for (int i = max(0, c - 2); i < c; ++i) poll(&cbfull[i & 1], (i >> 1) & 1);
+        for (int i = max(0, u - kXSlots); i < u; ++i) poll(&xfull[i % kXSlots], (i / kXSlots) & 1);
       }
     }
   } else if (warp == 1) {
-    // ---- MMAs
-    if (lane == 0) {
-      auto wait1 = [&](uint64_t* b, uint32_t parity) {
-        if (mbar_wait(b, parity, abort_flag)) return true;
-        if (!*abort_flag) atomicExch(p.err, kScanTimeout);
-        *abort_flag = 1;
-        return false;
-      };
-      auto scores = [&](int c) {  // G = C B^T
-        const int st = c & 1;
-        if (!wait1(&vfull[st], (c >> 1) & 1) || !wait1(&cbfull[st], (c >> 1) & 1)) return false;
+    // ---- the state's MMAs: H += (32 tokens of the split operand)^T B
+    bool ok = true;
+#pragma unroll 1
+    for (int c = 0; c < chunks; ++c) {
+      const int st = c & 1;
+      const uint64_t dB = desc_mn(sbase + st * K::STAGE + K::oB, kTile);
+      if (!(ok = wait(hready, c & 1) && wait(&cbfull[st], (c >> 1) & 1))) break;
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j) {
+        if (!(ok = wait(&xwfull[j & 1], j >> 1))) break;
         tc::fence_after();
-        const uint32_t a = sbase + st * K::STAGE + K::oC, b = sbase + st * K::STAGE + K::oB;
+        const uint64_t dj = tc::desc_at(dB, j * 32 * 128);
+        if (tc::elect()) {
 #pragma unroll
-        for (int k = 0; k < N / 16; ++k) {
-          const uint32_t off = (k / 4) * kTile + (k % 4) * 32;
-          mma_ss(tmem + cG, tc::desc_k(a + off), tc::desc_k(b + off), idesc_bf16(Q, false), k != 0);
-        }
-        tc::commit(gfull);
-        return true;
-      };
-      bool ok = ENDS || scores(0);
-      for (int c = 0; c < chunks && ok; ++c) {
-        const int st = c & 1;
-        const uint32_t sC = sbase + st * K::STAGE + K::oC, sB = sbase + st * K::STAGE + K::oB;
-        if (!wait1(hready, c & 1) || !wait1(&cbfull[st], (c >> 1) & 1)) break;
-        if (!ENDS) {
-          if (c > 0 && !wait1(yfree, (c - 1) & 1)) break;
-          tc::fence_after();
-#pragma unroll
-          for (int k = 0; k < N / 16; ++k) {  // Y = C H^T
-            const uint32_t off = (k / 4) * kTile + (k % 4) * 32;
-            mma_ss(tmem + cY, tc::desc_k(sC + off), tc::desc_k(sbase + K::oH + off), idesc_bf16(Q, false), k != 0);
-          }
-          tc::commit(y2full);
-        }
-        for (int j = 0; j < 6; ++j) {  // H += (split operand, half j / 3 of the tokens)^T B
-          const int n = 3 * c + (j >> 1);
-          if (!(ok = wait1(&xwfull[j & 1], n & 1))) break;
-          tc::fence_after();
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_ts(tmem + cH, tmem + cXW + (j & 1) * 32 + k * 8, desc_mn(sB + (j / 3) * 64 * 128 + k * 16 * 128, kTile),
+          for (int k = 0; k < 6; ++k)  // three splits, two steps of 16 tokens each
+            mma_ts(tmem + cH, tmem + cXW + (j & 1) * 64 + (k >> 1) * 16 + (k & 1) * 8, tc::desc_at(dj, (k & 1) * 16 * 128),
                    idesc_bf16(N, true), 1);
           tc::commit(&xwempty[j & 1]);
         }
-        if (!ok) break;
+        __syncwarp();
+      }
+      if (!ok) break;
+      if (tc::elect()) {
         tc::commit(hdone);
-        if (ENDS) {
-          tc::commit(&cbempty[st]);
-          continue;
-        }
-        if (!(ok = wait1(y2scaled, c & 1) && wait1(&xscan[st], (c >> 1) & 1))) break;
-        for (int h = 0; h < 2 && ok; ++h) {  // Y += S X
-          const int u = 2 * c + h, sl = u % kXSlots;
-          if (!(ok = wait1(&sfull[h], c & 1) && wait1(&xfull[sl], (u / kXSlots) & 1))) break;
-          tc::fence_after();
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mma_ts(tmem + cY + h * 64, tmem + (h ? cS1 : cS0) + k * 8, desc_mn(sbase + K::oX + sl * kTile + k * 16 * 128, kTile),
-                   idesc_bf16(64, true), 1);
-          tc::commit(&xempty[sl]);
-        }
-        if (!ok) break;
-        tc::commit(yfull);
         tc::commit(&cbempty[st]);
-        if (c + 1 < chunks) ok = scores(c + 1);
       }
-      tc::commit(done);  // the CTA leaves (and frees its TMEM) after the last MMA
-      volatile int never = 0;
-      mbar_wait(done, 0, &never);
+      __syncwarp();
     }
-  } else if (warp < 4) {
-    // ---- decays of head h0 + hh
-    const int hh = warp - 2, head = h0 + hh;
-    const bool has = head < p.heads;
-    const float a2 = has ? p.a[head] * 1.4426950408889634f : 0.f;
-    float raw[4];
-    auto fetch = [&](int c) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = c * Q + 4 * lane + k;
-        raw[k] = has && t.first + i < end ? p.dt[(long long)(t.first + i) * p.lddt + head] : 0.f;
+    if (tc::elect()) tc::commit(done);  // the CTA leaves (and frees its TMEM) after the last MMA
+    __syncwarp();
+    poll(done, 0);
+    if (!ok && lane == 0) failed();
+  } else if (warp == 3) {
+    // ---- y's MMAs: G = C B^T, Y = C H^T, Y += S X
+    if (!ENDS) {
+      const uint64_t dC0 = tc::desc_k(sbase + K::oC), dB0 = tc::desc_k(sbase + K::oB), dH = tc::desc_k(sbase + K::oH),
+                     dX0 = desc_mn(sbase + K::oX, kTile);
+      bool ok = true;
+#pragma unroll 1
+      for (int i = 0; i <= chunks; ++i) {
+        // Y of chunk i - 1, then G of chunk i
+        const int c = i - 1, st = c & 1;
+        if (i > 0) {
+          const uint64_t dC = tc::desc_at(dC0, st * K::STAGE);
+          if (!(ok = wait(hready, c & 1) && wait(&cbfull[st], (c >> 1) & 1) && (c == 0 || wait(yfree, (c - 1) & 1)))) break;
+          tc::fence_after();
+          if (tc::elect()) {
+#pragma unroll 2
+            for (int k = 0; k < N / 16; ++k) {
+              const uint32_t off = (k / 4) * kTile + (k % 4) * 32;
+              mma_ss(tmem + cY, tc::desc_at(dC, off), tc::desc_at(dH, off), idesc_bf16(Q, false), k != 0);
+            }
+            tc::commit(y2full);
+          }
+          __syncwarp();
+          if (!(ok = wait(sfull, c & 1) && wait(&xscan[c % kVecs], (c / kVecs) & 1) && wait(y2scaled, c & 1))) break;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            const int u = 2 * c + h, sl = u % kXSlots;
+            if (!(ok = wait(&xfull[sl], (u / kXSlots) & 1))) break;
+            tc::fence_after();
+            const uint64_t dX = tc::desc_at(dX0, sl * kTile);
+            if (tc::elect()) {
+#pragma unroll 4
+              for (int k = 0; k < 8; ++k)
+                mma_ts(tmem + cY + h * 64, tmem + s_col(h, k), tc::desc_at(dX, k * 16 * 128), idesc_bf16(64, true), 1);
+              tc::commit(&xempty[sl]);
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          if (tc::elect()) {
+            tc::commit(yfull);
+            tc::commit(&cbempty[st]);
+          }
+          __syncwarp();
+        }
+        if (i < chunks) {
+          if (!(ok = wait(&vfull[i % kVecs], (i / kVecs) & 1) && wait(&cbfull[i & 1], (i >> 1) & 1))) break;
+          tc::fence_after();
+          const uint64_t a = tc::desc_at(dC0, (i & 1) * K::STAGE), b = tc::desc_at(dB0, (i & 1) * K::STAGE);
+          if (tc::elect()) {
+#pragma unroll 2
+            for (int k = 0; k < N / 16; ++k) {
+              const uint32_t off = (k / 4) * kTile + (k % 4) * 32;
+              mma_ss(tmem + cG, tc::desc_at(a, off), tc::desc_at(b, off), idesc_bf16(Q, false), k != 0);
+            }
+            tc::commit(gfull);
+          }
+          __syncwarp();
+        }
       }
-    };
-    fetch(0);
+      if (tc::elect()) tc::commit(done);
+      __syncwarp();
+      poll(done, 0);
+      if (!ok && lane == 0) failed();
+    }
+  } else if (warp == 2) {
+    // ---- decays of both heads, four tokens a lane
+    bool ok = true;
+#pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
-      const int st = c & 1, valid = min(Q, end - t.first - c * Q);
-      float dt[4];
-      Pair cum[4];
+      const int st = c & 1, vs = c % kVecs, valid = min(Q, end - t.first - c * Q);
+      if (c >= kVecs && !(ok = wait(&vempty[vs], ((c / kVecs) & 1) ^ 1))) break;
+#pragma unroll 1
+      for (int hh = 0; hh < 2; ++hh) {
+        Vec& v = vec[vs * 2 + hh];
+        const bool has = h0 + hh < p.heads;
+        const float a2 = has ? p.a[h0 + hh] * 1.4426950408889634f : 0.f;
+        const float* at = p.dt + (long long)(t.first + c * Q + 4 * lane) * p.lddt + h0 + hh;
+        float dt[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const bool in = has && 4 * lane + k < valid;
-        dt[k] = in ? (p.softplus ? softplusf_(raw[k]) : raw[k]) : 0.f;
-        const Pair v{in ? a2 * dt[k] : 0.f, 0.f};
-        cum[k] = k ? add(cum[k - 1], v) : v;
+        for (int k = 0; k < 4; ++k) dt[k] = has && 4 * lane + k < valid ? at[k * p.lddt] : 0.f;
+        if (p.softplus) {
+#pragma unroll 1
+          for (int k = 0; k < 4; ++k) {  // in turn, through the first place
+            const float x = softplusf_(dt[0]);
+            dt[0] = dt[1];
+            dt[1] = dt[2];
+            dt[2] = dt[3];
+            dt[3] = x;
+          }
+        }
+        Pair cum[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool in = has && 4 * lane + k < valid;
+          dt[k] = in ? dt[k] : 0.f;
+          // Below 2^-200 a decay is zero in float32 whatever it multiplies; the
+          // bound keeps the sums small (and keeps a NaN).
+          float x = in ? a2 * dt[k] : 0.f;
+          asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(-200.f));
+          cum[k] = k ? add(cum[k - 1], {x, 0.f}) : Pair{x, 0.f};
+        }
+        Pair sum = cum[3];
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+          const Pair x = shfl_up(sum, o);
+          if (lane >= o) sum = add(x, sum);
+        }
+        Pair before = shfl_up(sum, 1);
+        if (lane == 0) before = {0.f, 0.f};
+        const Pair total = shfl(sum, 31), b1 = shfl(sum, 7), b2 = shfl(sum, 15), b3 = shfl(sum, 23);
+        const int blk = lane >> 3;
+        const Pair base = blk == 0 ? Pair{0.f, 0.f} : blk == 1 ? b1 : blk == 2 ? b2 : b3;
+        float o[5][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const Pair x = add(before, cum[k]);
+          o[0][k] = diff(base, x);
+          o[1][k] = ex2(diff(total, x)) * dt[k];
+          o[2][k] = ex2(diff(b1, x)) * dt[k];
+          o[3][k] = ex2(diff(b2, x)) * dt[k];
+          o[4][k] = ex2(diff(b3, x)) * dt[k];
+        }
+        auto put = [&](float* to, const float (&f)[4]) { reinterpret_cast<float4*>(to)[lane] = make_float4(f[0], f[1], f[2], f[3]); };
+        put(v.neg, o[0]);
+        put(v.dt, dt);
+        put(v.w, o[1]);
+        if (blk < 1) put(v.col, o[2]);
+        if (blk < 2) put(v.col + 32, o[3]);
+        if (blk < 3) put(v.col + 96, o[4]);
+        if ((lane & 7) == 0) v.base[blk] = base.hi + base.lo;
+        if (lane == 0) v.total = ex2(total.hi + total.lo);
       }
-      if (c + 1 < chunks) fetch(c + 1);
-      Pair sum = cum[3];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const Pair v = shfl_up(sum, o);
-        if (lane >= o) sum = add(v, sum);
-      }
-      Pair before = shfl_up(sum, 1);
-      if (lane == 0) before = {0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) cum[k] = add(before, cum[k]);
-      const Pair total = shfl(sum, 31), b1 = shfl(sum, 7), b2 = shfl(sum, 15), b3 = shfl(sum, 23);
-      const int blk = lane >> 3;
-      const Pair base = blk == 0 ? Pair{0.f, 0.f} : blk == 1 ? b1 : blk == 2 ? b2 : b3;
-      if (c >= 2 && !wait(&vempty[st], ((c >> 1) & 1) ^ 1)) break;
-      Vec& v = vec[st * 2 + hh];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int s = 4 * lane + k;
-        v.tok[s] = make_float4(cum[k].hi, cum[k].lo, dt[k], ex2(diff(total, cum[k])) * dt[k]);
-        v.start[s] = ex2(cum[k].hi + cum[k].lo);
-        v.row[s] = ex2(diff(cum[k], base));
-        if (blk < 1) v.col[s] = ex2(diff(b1, cum[k])) * dt[k];
-        if (blk < 2) v.col[32 + s] = ex2(diff(b2, cum[k])) * dt[k];
-        if (blk < 3) v.col[96 + s] = ex2(diff(b3, cum[k])) * dt[k];
-      }
-      if (lane == 0) v.total = ex2(total.hi + total.lo);
       if (valid < Q) {
         // Behind the sequence's end lie other sequences' rows: zeros, so that
         // nothing of them meets a product.
-        const int u = 2 * c + hh, sl = u % kXSlots;
-        if (!wait(&cbfull[st], (c >> 1) & 1) || !wait(&xfull[sl], (u / kXSlots) & 1)) break;
-        uint4* xr = reinterpret_cast<uint4*>(smem + K::oX + sl * kTile);
-        for (int i = valid * 8 + lane; i < Q * 8; i += 32) xr[i] = make_uint4(0, 0, 0, 0);
-        if (hh < NB) {
-          uint4* br = reinterpret_cast<uint4*>(smem + st * K::STAGE + K::oB + hh * kTile);
+        ok = wait(&cbfull[st], (c >> 1) & 1);
+#pragma unroll 1
+        for (int h = 0; h < 2 && ok; ++h) {
+          const int u = 2 * c + h, sl = u % kXSlots;
+          if (!(ok = wait(&xfull[sl], (u / kXSlots) & 1))) break;
+          uint4* xr = reinterpret_cast<uint4*>(smem + K::oX + sl * kTile);
+          for (int i = valid * 8 + lane; i < Q * 8; i += 32) xr[i] = make_uint4(0, 0, 0, 0);
+        }
+        if (!ok) break;
+        for (int n = 0; n < NB; ++n) {
+          uint4* br = reinterpret_cast<uint4*>(smem + st * K::STAGE + K::oB + n * kTile);
           for (int i = valid * 8 + lane; i < Q * 8; i += 32) br[i] = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async();
       }
-      arrive(&vfull[st]);
+      arrive(&vfull[vs]);
     }
-  } else if (warp < 8) {
-    // ---- S from G
+    if (!ok && lane == 0) failed();
+  } else if (warp < 12) {
+    // ---- S of both heads from G, in its place: lane = token t, the blocks of 16 tokens s in turn
     if (!ENDS) {
-      const int q = warp & 3, row = q * 32 + lane;
+      const int q = warp & 3, row = q * 32 + lane, odd = (warp >> 2) & 1;
+      bool ok = true;
+#pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
-        const int st = c & 1;
-        if (!wait(&vfull[st], (c >> 1) & 1) || !wait(gfull, c & 1)) break;
+        const int vs = c % kVecs;
+        if (!(ok = wait(&vfull[vs], (c / kVecs) & 1) && wait(gfull, c & 1))) break;
         tc::fence_after();
+        const int colbase = (q == 1 ? 0 : q == 2 ? 32 : 96);
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const Vec& v = vec[st * 2 + h];
-          const float rowf = v.row[row];
-          const float4 me = v.tok[row];
-          const float* col = v.col + (q == 1 ? 0 : q == 2 ? 32 : 96);
-          const uint32_t dst = tmem + lanes + (h ? cS1 : cS0);
+        for (int k = odd; k < 8; k += 2) {
+          const uint32_t at = tmem + lanes + cG + k * 16;
+          uint32_t r[16];
+          if (k >> 1 <= q) {
+            tc::tmem_ld16(at, r);
+            tc::tmem_wait_ld();
+            tc::landed(r);
+          }
 #pragma unroll 1
-          for (int j = 0; j < 4; ++j) {
-            uint32_t o[16];
-            if (j <= q) {
-              uint32_t r[32];
-              tc::tmem_ld32(tmem + lanes + cG + j * 32, r);
-              tc::tmem_wait_ld();
-              tc::landed(r);
-              if (j < q) {
+          for (int h = 0; h < 2; ++h) {
+            const Vec& v = vec[vs * 2 + h];
+            uint32_t o[8];
+            if (k >> 1 < q) {
+              const float rw = ex2(-v.neg[row]);
+              const F2 rw2 = f2(rw, rw);
+              const float* col = v.col + colbase + k * 16;
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                  const float4 f = *reinterpret_cast<const float4*>(col + j * 32 + i);
-                  o[i / 2] = pack_bf16(__uint_as_float(r[i]) * (f.x * rowf), __uint_as_float(r[i + 1]) * (f.y * rowf));
-                  o[i / 2 + 1] = pack_bf16(__uint_as_float(r[i + 2]) * (f.z * rowf), __uint_as_float(r[i + 3]) * (f.w * rowf));
-                }
-              } else {
+              for (int i = 0; i < 16; i += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(col + i);
+                o[i / 2] = pack_bf16(mul2(f2(r[i], r[i + 1]), mul2(f2(f.x, f.y), rw2)));
+                o[i / 2 + 1] = pack_bf16(mul2(f2(r[i + 2], r[i + 3]), mul2(f2(f.z, f.w), rw2)));
+              }
+            } else if (k >> 1 == q) {
+              // 32 tokens' sums stay below 6400, so a difference is exact to 2^-11, below S's own rounding
+              const float me = -v.neg[row];
+              const F2 me2 = f2(me, me);
+              const int last = lane - (k & 1) * 16;  // the row's own token in this block
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                  float e[2];
+              for (int i = 0; i < 16; i += 4) {
+                const float4 sn = *reinterpret_cast<const float4*>(v.neg + k * 16 + i);
+                const float4 sd = *reinterpret_cast<const float4*>(v.dt + k * 16 + i);
+                float e[4], w[4];
+                split(add2(me2, f2(sn.x, sn.y)), e[0], e[1]);
+                split(add2(me2, f2(sn.z, sn.w)), e[2], e[3]);
+                split(mul2(mul2(f2(ex2(e[0]), ex2(e[1])), f2(sd.x, sd.y)), f2(r[i], r[i + 1])), w[0], w[1]);
+                split(mul2(mul2(f2(ex2(e[2]), ex2(e[3])), f2(sd.z, sd.w)), f2(r[i + 2], r[i + 3])), w[2], w[3]);
 #pragma unroll
-                  for (int k = 0; k < 2; ++k) {
-                    const float4 s = v.tok[j * 32 + i + k];
-                    const float w = ex2((me.x - s.x) + (me.y - s.y)) * s.z;
-                    e[k] = i + k <= lane ? __uint_as_float(r[i + k]) * w : 0.f;
-                  }
-                  o[i / 2] = pack_bf16(e[0], e[1]);
-                }
+                for (int n = 0; n < 4; ++n) w[n] = i + n <= last ? w[n] : 0.f;  // s <= t, whatever G holds
+                o[i / 2] = pack_bf16(w[0], w[1]);
+                o[i / 2 + 1] = pack_bf16(w[2], w[3]);
               }
             } else {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = 0;
+              for (int i = 0; i < 8; ++i) o[i] = 0;
             }
-            tc::tmem_st16(dst + j * 16, o);
+            tc::tmem_st8(at + h * 8, o);
           }
-          tc::tmem_wait_st();
-          tc::fence_before();
-          arrive(&sfull[h]);
         }
-        arrive(&vempty[st]);
+        tc::tmem_wait_st();
+        tc::fence_before();
+        arrive(sfull);
+        arrive(&vempty[vs]);
       }
+      if (!ok && lane == 0) failed();
     }
-  } else if (warp < 12) {
-    // ---- the state: lane = row of the pair's 2 x 64
-    const int q = warp & 3, hh = q >> 1, pr = (q & 1) * 32 + lane, prow = q * 32 + lane, head = h0 + hh;
+  } else if (warp < 20) {
+    // ---- the state: lane = row of the pair's 2 x 64; its columns, and blocks of 32 tokens, in two halves
+    const int q = warp & 3, half = (warp >> 2) & 1 ? 0 : 1, hh = q >> 1, pr = (q & 1) * 32 + lane, prow = q * 32 + lane, head = h0 + hh;
     const bool has = head < p.heads;
     const long long hp = 64LL * N;
     float* own = p.ssm + ((long long)slot * p.heads + head) * hp + (long long)pr * N;
@@ -473,25 +574,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const float* from = g.seg > 0 ? part : own;
     uint8_t* hrow = smem + K::oH + prow * 128;
     bool ok = true;
-    for (int c = 0; c < chunks; ++c) {
-      const int st = c & 1, u = 2 * c + hh, sl = u % kXSlots;
-      if (!(ok = wait(&vfull[st], (c >> 1) & 1))) break;
-      if (c > 0 && !(ok = wait(hdone, (c - 1) & 1))) break;
-      if (c > 0 && !ENDS && !(ok = wait(y2full, (c - 1) & 1))) break;
-      tc::fence_after();
-      const Vec& v = vec[st * 2 + hh];
-      const float total = v.total;
 #pragma unroll 1
-      for (int j = 0; j < N / 32; ++j) {
-        uint32_t r[32];
+    for (int c = 0; c < chunks; ++c) {
+      const int vs = c % kVecs, u = 2 * c + hh, sl = u % kXSlots;
+      if (!(ok = wait(&vfull[vs], (c / kVecs) & 1) && (c == 0 || (wait(hdone, (c - 1) & 1) && (ENDS || wait(y2full, (c - 1) & 1)))))) break;
+      tc::fence_after();
+      const Vec& v = vec[vs * 2 + hh];
+      const F2 total = f2(v.total, v.total);
+#pragma unroll 1
+      for (int j = half * (N / 32); j < (half + 1) * (N / 32); ++j) {
+        uint32_t r[16];
         if (c > 0) {
-          tc::tmem_ld32(tmem + lanes + cH + j * 32, r);
+          tc::tmem_ld16(tmem + lanes + cH + j * 16, r);
           tc::tmem_wait_ld();
           tc::landed(r);
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 f = !ENDS && has ? *reinterpret_cast<const float4*>(from + j * 32 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int i = 0; i < 16; i += 4) {
+            const float4 f = !ENDS && has ? *reinterpret_cast<const float4*>(from + j * 16 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
             r[i] = __float_as_uint(f.x);
             r[i + 1] = __float_as_uint(f.y);
             r[i + 2] = __float_as_uint(f.z);
@@ -500,19 +600,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (!ENDS) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
+          for (int i = 0; i < 16; i += 8) {
             uint4 o;
             o.x = pack_bf16(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
             o.y = pack_bf16(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
             o.z = pack_bf16(__uint_as_float(r[i + 4]), __uint_as_float(r[i + 5]));
             o.w = pack_bf16(__uint_as_float(r[i + 6]), __uint_as_float(r[i + 7]));
-            const int chunk = (j & 1) * 4 + i / 8;
-            *reinterpret_cast<uint4*>(hrow + (j >> 1) * kTile + ((chunk ^ (prow & 7)) << 4)) = o;
+            const int chunk = (j & 3) * 2 + i / 8;
+            *reinterpret_cast<uint4*>(hrow + (j >> 2) * kTile + ((chunk ^ (prow & 7)) << 4)) = o;
           }
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * total);
-        tc::tmem_st32(tmem + lanes + cH + j * 32, r);
+        for (int i = 0; i < 16; i += 2) {
+          float x, y;
+          split(mul2(f2(r[i], r[i + 1]), total), x, y);
+          r[i] = __float_as_uint(x);
+          r[i + 1] = __float_as_uint(y);
+        }
+        tc::tmem_st16(tmem + lanes + cH + j * 16, r);
       }
       tc::tmem_wait_st();
       if (!ENDS) fence_proxy_async();
@@ -521,46 +626,57 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // exp(c[T] - c[s]) dt[s] x[s], split over three bf16 values, tokens along the columns
       if (!(ok = wait(&xfull[sl], (u / kXSlots) & 1))) break;
       const uint8_t* xs = smem + K::oX + sl * kTile + (pr & 7) * 2;
-      float finite = 0.f;
+      F2 finite = f2(0.f, 0.f);
+      const F2 zero = finite, minus = f2(-1.f, -1.f);
 #pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        uint32_t o[3][32];
+      for (int i4 = 0; i4 < 4; ++i4) {  // 16 tokens; 32 fill a buffer
+        const int j = half * 2 + (i4 >> 1) * 4 + (i4 & 1);  // of the chunk's eight
+        if (!(i4 & 1)) {
+          if ((c > 0 || i4 > 0) && !(ok = wait(&xwempty[half], (i4 >> 1) ^ 1))) break;
+          tc::fence_after();
+        }
+        uint32_t o[3][8];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int s = half * 64 + 2 * i;
-          const float x0 = __uint_as_float(uint32_t(*reinterpret_cast<const uint16_t*>(xs + s * 128 + (((pr >> 3) ^ (s & 7)) << 4))) << 16);
-          const float x1 =
-              __uint_as_float(uint32_t(*reinterpret_cast<const uint16_t*>(xs + (s + 1) * 128 + (((pr >> 3) ^ ((s + 1) & 7)) << 4))) << 16);
-          finite = fmaf(x0, 0.f, finite);
-          finite = fmaf(x1, 0.f, finite);
-          float f0 = x0 * v.tok[s].w, f1 = x1 * v.tok[s + 1].w;
-          o[0][i] = pack_bf16(f0, f1);
-          f0 -= bf_lo(o[0][i]);
-          f1 -= bf_hi(o[0][i]);
-          o[1][i] = pack_bf16(f0, f1);
-          f0 -= bf_lo(o[1][i]);
-          f1 -= bf_hi(o[1][i]);
-          o[2][i] = pack_bf16(f0, f1);
+        for (int i = 0; i < 8; i += 2) {
+          const int s = j * 16 + 2 * i;
+          const float4 w = *reinterpret_cast<const float4*>(v.w + s);
+          float x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // s is a multiple of four: the swizzle of row s + k by constants alone
+            x[k] = __uint_as_float(uint32_t(*reinterpret_cast<const uint16_t*>(xs + (s + k) * 128 + (((pr >> 3) ^ ((2 * i + k) & 7)) << 4))) << 16);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const F2 xx = f2(x[2 * k], x[2 * k + 1]);
+            finite = fma2(xx, zero, finite);
+            F2 f = mul2(xx, k ? f2(w.z, w.w) : f2(w.x, w.y));
+            const uint32_t a = pack_bf16(f);
+            f = fma2(f2(bf_lo(a), bf_hi(a)), minus, f);
+            const uint32_t b = pack_bf16(f);
+            f = fma2(f2(bf_lo(b), bf_hi(b)), minus, f);
+            o[0][i + k] = a;
+            o[1][i + k] = b;
+            o[2][i + k] = pack_bf16(f);
+          }
         }
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const int j = 3 * half + k, n = 3 * c + (j >> 1);  // n: uses of buffer j & 1 before this one
-          if (n > 0 && !(ok = wait(&xwempty[j & 1], (n - 1) & 1))) break;
-          tc::fence_after();
-          tc::tmem_st32(tmem + lanes + cXW + (j & 1) * 32, o[k]);
+        for (int k = 0; k < 3; ++k) tc::tmem_st8(tmem + lanes + cXW + half * 64 + k * 16 + (i4 & 1) * 8, o[k]);
+        if (i4 & 1) {
           tc::tmem_wait_st();
           tc::fence_before();
-          arrive(&xwfull[j & 1]);
+          arrive(&xwfull[half]);
         }
-        if (!ok) break;
       }
       if (!ok) break;
       if (!ENDS) {
         // A value of x that is not finite would reach earlier tokens' y through
         // the zeros of S: it leaves the tile, and y from its token on is NaN.
         int first = Q;
-        if (finite != 0.f) {
+        float f0, f1;
+        split(finite, f0, f1);
+        if (f0 + f1 != 0.f) {
+#pragma unroll 1
           for (int s = Q - 1; s >= 0; --s) {
+            if (((s >> 5) & 1) != half) continue;
             uint16_t* e = reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(xs) + s * 128 + (((pr >> 3) ^ (s & 7)) << 4));
             if ((*e & 0x7f80) == 0x7f80) {
               first = s;
@@ -569,126 +685,134 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           fence_proxy_async();
         }
-        bad[st * 128 + prow] = first;
+        bad[(vs * 2 + half) * 128 + prow] = uint8_t(first);
         const bool any = __any_sync(0xffffffffu, first < Q);
-        if (lane == 0) anybad[st * 4 + q] = any;
-        arrive(&xscan[st]);
+        if (lane == 0) anybad[vs * 8 + half * 4 + q] = any;
+        arrive(&xscan[vs]);
       }
       arrive(&xempty[sl]);
-      arrive(&vempty[st]);
+      arrive(&vempty[vs]);
     }
-    if (ok && wait(hdone, (chunks - 1) & 1) && (ENDS || end == t.end)) {
+    if (ok) ok = wait(hdone, (chunks - 1) & 1);
+    if (!ok && lane == 0) failed();
+    if (ok && (ENDS || end == t.end)) {
       tc::fence_after();
       float* to = ENDS ? part : own;
 #pragma unroll 1
-      for (int j = 0; j < N / 32; ++j) {
-        uint32_t r[32];
-        tc::tmem_ld32(tmem + lanes + cH + j * 32, r);
+      for (int j = half * (N / 32); j < (half + 1) * (N / 32); ++j) {
+        uint32_t r[16];
+        tc::tmem_ld16(tmem + lanes + cH + j * 16, r);
         tc::tmem_wait_ld();
         tc::landed(r);
         if (has) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(to + j * 32 + i) =
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(to + j * 16 + i) =
                 make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
         }
       }
     }
   } else if (!ENDS) {
-    // ---- y: lane = token
-    const int q = warp & 3, row = q * 32 + lane;
-    for (int c = 0; c < chunks; ++c) {
-      const int st = c & 1, valid = min(Q, end - t.first - c * Q);
-      const long long tok = t.first + c * Q + row;
-      if (!wait(&vfull[st], (c >> 1) & 1) || !wait(y2full, c & 1)) break;
-      tc::fence_after();
+    // ---- y of one head: lane = token
+    const int q = warp & 3, row = q * 32 + lane, h = (warp - 20) >> 2, head = h0 + h;
+    const bool has = head < p.heads;
+    const float d = has && p.d ? p.d[head] : 0.f;
+    const F2 d2 = f2(d, d), l2e = f2(-1.4426950408889634f, -1.4426950408889634f), one = f2(1.f, 1.f);
+    const uint32_t ycol = tmem + lanes + cY + h * 64;
+    bool ok = true;
 #pragma unroll 1
-      for (int j = 0; j < 4; ++j) {
-        const float f = vec[st * 2 + (j >> 1)].start[row];
-        uint32_t r[32];
-        tc::tmem_ld32(tmem + lanes + cY + j * 32, r);
+    for (int c = 0; c < chunks; ++c) {
+      const int vs = c % kVecs, u = 2 * c + h, sl = u % kXSlots;
+      const long long tok = t.first + c * Q + row;
+      const bool in = has && t.first + c * Q + row < end;
+      uint32_t z[32];
+      if (p.z && in) {  // in flight while the products run
+        const uint16_t* zp = reinterpret_cast<const uint16_t*>(p.z) + tok * p.ldz + head * 64;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+          asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                       : "=r"(z[i]), "=r"(z[i + 1]), "=r"(z[i + 2]), "=r"(z[i + 3]), "=r"(z[i + 4]), "=r"(z[i + 5]),
+                         "=r"(z[i + 6]), "=r"(z[i + 7])
+                       : "l"(zp + 2 * i));
+      }
+      if (!(ok = wait(&vfull[vs], (c / kVecs) & 1) && wait(&xfull[sl], (u / kXSlots) & 1) && wait(y2full, c & 1))) break;
+      tc::fence_after();
+      const Vec& v = vec[vs * 2 + h];
+      const float f = ex2(v.base[q] - v.neg[row]);
+      const F2 ff = f2(f, f);
+      const uint8_t* xr = smem + K::oX + sl * kTile + row * 128;
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j) {  // exp(c[t]) C H^T + d x
+        uint32_t r[16];
+        tc::tmem_ld16(ycol + j * 16, r);
+        const uint4 x0 = *reinterpret_cast<const uint4*>(xr + (((j * 2) ^ (row & 7)) << 4));
+        const uint4 x1 = *reinterpret_cast<const uint4*>(xr + (((j * 2 + 1) ^ (row & 7)) << 4));
+        const uint32_t xw[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
         tc::tmem_wait_ld();
         tc::landed(r);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
-        tc::tmem_st32(tmem + lanes + cY + j * 32, r);
+        for (int i = 0; i < 8; ++i) {
+          float x, y;
+          split(fma2(f2(r[2 * i], r[2 * i + 1]), ff, mul2(d2, f2(bf_lo(xw[i]), bf_hi(xw[i])))), x, y);
+          r[2 * i] = __float_as_uint(x);
+          r[2 * i + 1] = __float_as_uint(y);
+        }
+        tc::tmem_st16(ycol + j * 16, r);
       }
       tc::tmem_wait_st();
       tc::fence_before();
       arrive(y2scaled);
-      bool ok = true;
+      arrive(&xempty[sl]);
+      if (!(ok = wait(yfull, c & 1) && wait(&xscan[vs], (c / kVecs) & 1))) break;
+      tc::fence_after();
+      const int spoilt = anybad[vs * 8 + 2 * h] | anybad[vs * 8 + 2 * h + 1] | anybad[vs * 8 + 4 + 2 * h] | anybad[vs * 8 + 4 + 2 * h + 1];
 #pragma unroll 1
-      for (int j = 0; j < 4; ++j) {  // 32 columns: half j & 1 of head j >> 1
-        const int h = j >> 1, head = h0 + h, u = 2 * c + h, sl = u % kXSlots;
-        const bool in = row < valid && head < p.heads;
-        uint4 z[4];
-        if (p.z && in) {  // in flight while the products finish
-          const uint4* zp = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.z) + tok * p.ldz + head * 64 + (j & 1) * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) z[i] = __ldcs(zp + i);
-        }
-        if (j == 0 && !(ok = wait(yfull, c & 1) && wait(&xscan[st], (c >> 1) & 1))) break;
-        if (!(j & 1) && !(ok = wait(&xfull[sl], (u / kXSlots) & 1))) break;
-        tc::fence_after();
-        uint32_t r[32];
-        tc::tmem_ld32(tmem + lanes + cY + j * 32, r);
+      for (int j = 0; j < 4; ++j) {
+        uint32_t r[16];
+        tc::tmem_ld16(ycol + j * 16, r);
         tc::tmem_wait_ld();
         tc::landed(r);
         if (j == 3) {
           tc::fence_before();
           arrive(yfree);
         }
-        if (p.d && head < p.heads) {
-          const float d = p.d[head];
-          const uint8_t* xr = smem + K::oX + sl * kTile + row * 128;
+        uint32_t o[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 x = *reinterpret_cast<const uint4*>(xr + ((((j & 1) * 4 + i) ^ (row & 7)) << 4));
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        for (int k = 0; k < 8; ++k) {
+          F2 y = f2(r[2 * k], r[2 * k + 1]);
+          if (p.z) {  // y z / (1 + exp(-z))
+            const F2 zz = f2(bf_lo(z[k]), bf_hi(z[k]));
+            float e0, e1;
+            split(mul2(zz, l2e), e0, e1);
+            split(add2(f2(ex2(e0), ex2(e1)), one), e0, e1);
+            y = mul2(y, mul2(zz, f2(rcp(e0), rcp(e1))));
+          }
+          o[k] = pack_bf16(y);
+        }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              r[i * 8 + k * 2] = __float_as_uint(fmaf(d, bf_lo(w[k]), __uint_as_float(r[i * 8 + k * 2])));
-              r[i * 8 + k * 2 + 1] = __float_as_uint(fmaf(d, bf_hi(w[k]), __uint_as_float(r[i * 8 + k * 2 + 1])));
-            }
+        for (int i = 0; i < 24; ++i) z[i] = z[i + 8];  // the next columns' to the front
+        if (spoilt) {
+#pragma unroll 1
+          for (int i = 0; i < 16; ++i) {
+            const int first = min(bad[vs * 256 + h * 64 + j * 16 + i], bad[vs * 256 + 128 + h * 64 + j * 16 + i]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (k == i / 2 && row >= first) o[k] |= i & 1 ? 0x7fff0000u : 0x7fffu;
           }
         }
-        if (j & 1) arrive(&xempty[sl]);
-        if (p.z && in) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t w[4] = {z[i].x, z[i].y, z[i].z, z[i].w};
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float zz = k & 1 ? bf_hi(w[k / 2]) : bf_lo(w[k / 2]);
-              r[i * 8 + k] = __float_as_uint(__uint_as_float(r[i * 8 + k]) * __fdividef(zz, 1.0f + __expf(-zz)));
-            }
-          }
-        }
-        if (anybad[st * 4 + 2 * h] | anybad[st * 4 + 2 * h + 1]) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (row >= bad[st * 128 + j * 32 + i]) r[i] = 0x7fc00000u;
-        }
-        if (in) {
-          uint16_t* yp = reinterpret_cast<uint16_t*>(p.y) + tok * p.ldy + head * 64 + (j & 1) * 32;
-#pragma unroll
-          for (int i = 0; i < 32; i += 16) {
-            uint32_t o[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = pack_bf16(__uint_as_float(r[i + 2 * k]), __uint_as_float(r[i + 2 * k + 1]));
-            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(yp + i), "r"(o[0]), "r"(o[1]), "r"(o[2]),
-                         "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
-                         : "memory");
-          }
-        }
+        if (in)
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(reinterpret_cast<uint16_t*>(p.y) + tok * p.ldy +
+                                                                                head * 64 + j * 16),
+                       "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
+                       : "memory");
       }
-      if (!ok) break;
-      arrive(&vempty[st]);
+      arrive(&vempty[vs]);
     }
+    if (!ok && lane == 0) failed();
   }
   // log of the segment's decay, for the join: the same float32 sums, segment-wide
-  if (ENDS && warp >= 2 && warp < 4) {
-    const int head = h0 + warp - 2;
+  if (ENDS && warp >= 20 && warp < 22) {
+    const int head = h0 + warp - 20;
     if (head < p.heads) {
       Pair s{0.f, 0.f};
       for (int i = t.first + lane; i < end; i += 32) {
@@ -739,7 +863,7 @@ void run(const ScanParams& p, int seg, cudaStream_t s) {
 bool scan_tc_eligible(const ScanParams& p) {
   return p.type == kBF16 && p.size == 64 && (p.state == 64 || p.state == 128) && p.plan.longest >= 32 && aligned(p.x, 16) &&
          aligned(p.b, 16) && aligned(p.c, 16) && aligned(p.y, 32) && p.ldx % 8 == 0 && p.ldb % 8 == 0 && p.ldc % 8 == 0 &&
-         p.ldy % 16 == 0 && (!p.z || (aligned(p.z, 16) && p.ldz % 8 == 0));
+         p.ldy % 16 == 0 && (!p.z || (aligned(p.z, 32) && p.ldz % 16 == 0));
 }
 
 void scan_tc(const ScanParams& p, int seg, cudaStream_t s) {

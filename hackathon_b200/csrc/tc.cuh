@@ -29,6 +29,19 @@ __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
          (uint64_t(2) << 61);
 }
 
+// One lane of a converged warp. MMAs and commits are issued under it in code that
+// the whole warp runs, which leaves their descriptors in uniform registers: under
+// a test of the lane instead, each MMA of a chain took 100 to 200 cycles to issue
+// against the 32 to 128 it runs.
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Descriptors `bytes` further on (the address is the low field, in 16 bytes).
+__device__ __forceinline__ uint64_t desc_at(uint64_t d, uint32_t bytes) { return d + (bytes >> 4); }
+
 __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
@@ -64,6 +77,10 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t* r) {
       "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : B2E_R16(r, 0), B2E_R16(r, 16)
       : "r"(t));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::B2E_I4(r, 0), B2E_I4(r, 4), "r"(t)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t* r) {
