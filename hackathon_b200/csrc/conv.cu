@@ -5,7 +5,7 @@
 //   v = window[slot] ++ x[sequence];  y[t] = act(bias + sum_j w[j] v[t + j]);  window[slot] <- last taps - 1 of v
 //
 // Bound by HBM: each x and y once, a window once each way. A warp takes 32
-// vectors of channels (16 bytes of x a lane) over a tile of tokens and keeps the
+// vectors of four channels over a tile of tokens and keeps the
 // last taps - 1 inputs in registers, so a token is read once and a tile reads
 // only taps - 1 inputs of its neighbour's again. The tile that starts a
 // sequence is the only one that reads the window, and it writes it too: no
@@ -27,10 +27,10 @@ __device__ __forceinline__ void load_vec(const void* p, long long i, float (&v)[
     const float4 a = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i));
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   } else {
-    const uint4 r = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i));
-    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+    const uint2 r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + i));
+    const uint32_t u[2] = {r.x, r.y};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       if constexpr (T == kBF16) {
         v[2 * j] = __uint_as_float(u[j] << 16);
         v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
@@ -50,9 +50,9 @@ __device__ __forceinline__ void store_vec(void* p, long long i, const float (&v)
   } else if constexpr (T == kF32) {
     __stcs(reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i), make_float4(v[0], v[1], v[2], v[3]));
   } else {
-    uint32_t u[4];
+    uint32_t u[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       if constexpr (T == kBF16) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
         u[j] = *reinterpret_cast<const uint32_t*>(&h);
@@ -61,7 +61,7 @@ __device__ __forceinline__ void store_vec(void* p, long long i, const float (&v)
         u[j] = *reinterpret_cast<const uint32_t*>(&h);
       }
     }
-    __stcs(reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p) + i), make_uint4(u[0], u[1], u[2], u[3]));
+    __stcs(reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i), make_uint2(u[0], u[1]));
   }
 }
 
@@ -103,18 +103,13 @@ __device__ __forceinline__ float silu_fast(float v) { return __fdividef(v, 1.0f 
 
 template <int T, int VC, int TAPS>
 __global__ void __launch_bounds__(32 * kConvWarps) k_conv(const ConvParams p, int len, int vblocks, long long warps) {
-  constexpr int W = TAPS - 1, U = VC == 8 ? 4 : 8;  // tokens whose loads are in flight together
+  constexpr int W = TAPS - 1, U = 8;  // tokens whose loads are in flight together
   const long long gw = (long long)blockIdx.x * kConvWarps + (threadIdx.x >> 5);
   if (gw >= warps) return;
   const int tile = int(gw / vblocks), lane = threadIdx.x & 31;
   const int c = (int(gw % vblocks) * 32 + lane) * VC;
-  SeqTile t;
-  if (p.plan.starts) {
-    t = seq_tile(p.plan, tile, len);
-    if (!t.live && p.err && t.start < t.end && (t.start < 0 || t.end > p.plan.tokens)) *p.err = 1;
-  } else {
-    t = {tile, tile, tile + 1, tile, true};
-  }
+  const SeqTile t = seq_tile(p.plan, tile, len);
+  if (!t.live && p.err && t.start < t.end && (t.start < 0 || t.end > p.plan.tokens)) *p.err = 1;
   if (!t.live || c >= p.channels) return;
   const int slot = p.plan.slots ? p.plan.slots[t.seq] : t.seq;
   if (slot < 0 || slot >= p.plan.state_rows) {
@@ -188,22 +183,76 @@ __global__ void __launch_bounds__(32 * kConvWarps) k_conv(const ConvParams p, in
   }
 }
 
+// One token a sequence: the windows' bytes count. A warp takes kStepSeqs
+// sequences for its channels, so that the weights are read once for them and
+// all their windows are in flight together.
+constexpr int kStepSeqs = 4;
+
+template <int T, int VC, int TAPS>
+__global__ void __launch_bounds__(32 * kConvWarps) k_conv_step(const ConvParams p, int vblocks, long long warps) {
+  constexpr int W = TAPS - 1;
+  const long long gw = (long long)blockIdx.x * kConvWarps + (threadIdx.x >> 5);
+  const int c = (int(gw % vblocks) * 32 + int(threadIdx.x & 31)) * VC, s0 = int(gw / vblocks) * kStepSeqs;
+  if (gw >= warps || c >= p.channels) return;
+  float old[kStepSeqs][VC][W], in[kStepSeqs][VC];
+  long long at[kStepSeqs];
+#pragma unroll
+  for (int i = 0; i < kStepSeqs; ++i) {
+    const int s = s0 + i;
+    int slot = -1;
+    if (s < p.plan.seqs) {
+      slot = p.plan.slots ? p.plan.slots[s] : s;
+      if (slot < 0 || slot >= p.plan.state_rows) {
+        slot = -1;
+        if (p.err) *p.err = 1;
+      }
+    }
+    at[i] = slot < 0 ? -1 : ((long long)slot * p.channels + c) * W;
+    if (slot >= 0) {
+      load_rows<VC, W>(p.window + at[i], old[i]);
+      load_vec<T, VC>(p.x, s * p.ldx + c, in[i]);
+    }
+  }
+  float w[VC][TAPS], bias[VC];
+  load_rows<VC, TAPS>(p.w + (long long)c * TAPS, w);
+#pragma unroll
+  for (int i = 0; i < VC; ++i) bias[i] = p.bias ? p.bias[c + i] : 0.f;
+#pragma unroll
+  for (int i = 0; i < kStepSeqs; ++i) {
+    if (at[i] < 0) continue;
+    float y[VC];
+#pragma unroll
+    for (int k = 0; k < VC; ++k) {
+      float s = bias[k];
+#pragma unroll
+      for (int j = 0; j < W; ++j) s = fmaf(w[k][j], old[i][k][j], s);
+      s = fmaf(w[k][W], in[i][k], s);
+      y[k] = p.silu ? silu_fast(s) : s;
+#pragma unroll
+      for (int j = 0; j + 1 < W; ++j) old[i][k][j] = old[i][k][j + 1];
+      old[i][k][W - 1] = in[i][k];
+    }
+    store_vec<T, VC>(p.y, (s0 + i) * p.ldy + c, y);
+    store_rows<VC, W>(p.window + at[i], old[i]);
+  }
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <int T, int VC, int TAPS>
 void launch(const ConvParams& p, cudaStream_t s) {
   const int vblocks = ceil_div(p.channels, 32 * VC);
-  int len = 1;
-  long long tiles = p.plan.seqs;
-  if (p.plan.starts) {
-    // Tiles of 32 tokens read 3 of them again; short tiles where long ones
-    // would leave the SMs without enough loads in flight.
-    len = (long long)p.plan.tokens * vblocks >= 32LL * 148 * 16 ? 32 : 8;
-    tiles = seq_tiles(p.plan, len);
-  }
-  const long long warps = tiles * vblocks, grid = (warps + kConvWarps - 1) / kConvWarps;
+  const bool step = p.plan.starts == nullptr;
+  // Tiles of 32 tokens read 3 of them again; short tiles where long ones would
+  // leave the SMs without enough loads in flight.
+  const int len = (long long)p.plan.tokens * vblocks >= 32LL * 148 * 16 ? 32 : 8;
+  const long long warps = (step ? ceil_div(p.plan.seqs, kStepSeqs) : seq_tiles(p.plan, len)) * vblocks;
+  const long long grid = (warps + kConvWarps - 1) / kConvWarps;
   B2E_CHECK(grid <= 0x7fffffffLL, kErrInvalid, "causal_conv: too many tiles");
-  k_conv<T, VC, TAPS><<<unsigned(grid), 32 * kConvWarps, 0, s>>>(p, len, vblocks, warps);
+  if (step)
+    k_conv_step<T, VC, TAPS><<<unsigned(grid), 32 * kConvWarps, 0, s>>>(p, vblocks, warps);
+  else
+    k_conv<T, VC, TAPS><<<unsigned(grid), 32 * kConvWarps, 0, s>>>(p, len, vblocks, warps);
   B2E_CUDA(cudaGetLastError());
 }
 
@@ -216,8 +265,9 @@ void launch_taps(const ConvParams& p, cudaStream_t s) {
 
 template <int T>
 void launch_type(const ConvParams& p, cudaStream_t s) {
-  constexpr int VC = T == kF32 ? 4 : 8;
-  const bool vec = p.channels % VC == 0 && p.ldx % VC == 0 && p.ldy % VC == 0 && aligned16(p.x) && aligned16(p.y) &&
+  constexpr int VC = 4;
+  const auto aligned = [](const void* v) { return (reinterpret_cast<uintptr_t>(v) & (VC * (T == kF32 ? 4 : 2) - 1)) == 0; };
+  const bool vec = p.channels % VC == 0 && p.ldx % VC == 0 && p.ldy % VC == 0 && aligned(p.x) && aligned(p.y) &&
                    aligned16(p.w) && aligned16(p.window);
   if (vec)
     launch_taps<T, VC>(p, s);

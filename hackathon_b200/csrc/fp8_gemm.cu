@@ -14,7 +14,7 @@
 //  - rows kernel: M = 128 activation rows (a thread's TMEM lane is a row, so both
 //    scales are one scalar a thread and group), N = BN output features;
 //    persistent CTAs. Bound by the tensor cores: a group costs 128 x BN x 128
-//    products, its epilogue BN/2 FMAs a thread of eight warps.
+//    products, its epilogue BN / 2 FMAs a thread of eight warps.
 //  - few-rows kernel: M = 128 output features, N = BR <= 64 rows; the groups are
 //    shared out over a cluster of up to 8 CTAs, whose float32 sums meet through
 //    distributed shared memory in rank order (the same result every time). Bound
@@ -30,8 +30,6 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kEpi = 8;                       // epilogue warps
-constexpr int kThreads = 64 + 32 * kEpi;      // TMA warp, MMA warp, epilogue
 constexpr uint32_t kKB = kFp8Group;           // bytes of a K step
 enum Fp8Error : int { kFp8TimeoutTma = 121, kFp8TimeoutMma = 122, kFp8TimeoutEpi = 123 };
 
@@ -61,48 +59,75 @@ struct Args {
   int* err;
 };
 
-// Eight float results to a row of y, n % 8 == 0, all inside.
-__device__ __forceinline__ void store8_y(const Args& e, long long at, const float (&v)[8]) {
-  if (e.y_type == kF32) {
-    float* p = reinterpret_cast<float*>(e.y) + at;
-    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
-                 "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
-                 : "memory");
-  } else {
-    uint32_t u[4];
+// ReLU that keeps a NaN.
+__device__ __forceinline__ float2 activate(float2 v, int relu) {
+  if (relu) {
+    v.x = v.x < 0.f ? 0.f : v.x;
+    v.y = v.y < 0.f ? 0.f : v.y;
+  }
+  return v;
+}
+
+// Sixteen results (two and two) to a row of y, all inside, 32-byte aligned.
+template <int Y>
+__device__ __forceinline__ void store16_y(void* y, long long at, const float2* v) {
+  if constexpr (Y == kF32) {
+    float* p = reinterpret_cast<float*>(y) + at;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (e.y_type == kBF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-        u[j] = *reinterpret_cast<const uint32_t*>(&h);
+    for (int i = 0; i < 8; i += 4)
+      asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p + 2 * i), "f"(v[i].x), "f"(v[i].y), "f"(v[i + 1].x),
+                   "f"(v[i + 1].y), "f"(v[i + 2].x), "f"(v[i + 2].y), "f"(v[i + 3].x), "f"(v[i + 3].y)
+                   : "memory");
+  } else {
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (Y == kBF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[i].x, v[i].y);
+        u[i] = *reinterpret_cast<const uint32_t*>(&h);
       } else {
-        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-        u[j] = *reinterpret_cast<const uint32_t*>(&h);
+        const __half2 h = __floats2half2_rn(v[i].x, v[i].y);
+        u[i] = *reinterpret_cast<const uint32_t*>(&h);
       }
     }
-    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(e.y) + at) = make_uint4(u[0], u[1], u[2], u[3]);
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(reinterpret_cast<uint16_t*>(y) + at), "r"(u[0]),
+                 "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                 : "memory");
   }
 }
 
 // ------------------------------------------------------------- rows kernel
+
+// Row scales come in blocks of kXB groups through shared memory, group-major: a
+// row's scales are contiguous in memory, so a load for every row of a tile takes
+// a line a lane, which per group cost more than the group's MMAs.
+constexpr int kXB = 16, kXStride = 128 + 1;
 
 template <int BN>
 struct RowsCfg {
   static constexpr uint32_t TILE_X = 128 * kKB, TILE_W = BN * kKB, STAGE = TILE_X + TILE_W;
   static constexpr int STAGES = BN == 256 ? 4 : 3;
   static constexpr int CTAS = BN == 256 ? 1 : 2;  // resident on an SM
+  // Eight epilogue warps behind a warpgroup of TMA, MMA and two idle warps. The
+  // registers are split by warpgroup: 4 x 32 x LOW + 8 x 32 x HIGH are the launch's
+  // 384 x 168 (80 where two CTAs share an SM).
+  static constexpr int EPI = 8, THREADS = 128 + 32 * EPI, HN = BN / 2;
+  static constexpr int LOW = BN == 256 ? 40 : 24, HIGH = BN == 256 ? 232 : 104;
+  static_assert(4 * LOW + 8 * HIGH <= 12 * (BN == 256 ? 168 : 80), "register shares exceed the launch's");
   static constexpr uint32_t TMEM = 2 * BN;
-  static constexpr size_t SMEM = size_t(STAGES) * STAGE + 1024 + 256;
+  static constexpr uint32_t SCALES = kXB * kXStride * 4;  // row scales of kXB groups
+  static constexpr size_t SMEM = size_t(STAGES) * STAGE + SCALES + 1024 + 256;
 };
 
-template <int BN>
-__global__ void __launch_bounds__(kThreads, RowsCfg<BN>::CTAS)
+template <int BN, int Y>
+__global__ void __launch_bounds__(RowsCfg<BN>::THREADS, RowsCfg<BN>::CTAS)
     k_fp8_rows(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, const Args e) {
   using K = RowsCfg<BN>;
-  constexpr int S = K::STAGES, HN = BN / 2;
+  constexpr int S = K::STAGES, HN = K::HN;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + size_t(S) * K::STAGE);
+  float* xsm = reinterpret_cast<float*>(smem + size_t(S) * K::STAGE);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + size_t(S) * K::STAGE + K::SCALES);
   uint64_t* empty = full + S;
   uint64_t* pfull = empty + S;   // a group's sum is in TMEM buffer b
   uint64_t* pempty = pfull + 2;  // its epilogue has read it
@@ -117,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, RowsCfg<BN>::CTAS)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&pfull[b], 1);
-      mbar_init(&pempty[b], kEpi);
+      mbar_init(&pempty[b], K::EPI);
     }
     mbar_init(done, 1);
     *abort_flag = 0;
@@ -133,6 +158,8 @@ __global__ void __launch_bounds__(kThreads, RowsCfg<BN>::CTAS)
   const uint32_t tmem = *tmem_slot;
   const int tiles = e.tiles_m * e.tiles_n;
 
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(K::LOW));
   if (warp == 0) {
     if (lane == 0) {
       int it = 0;
@@ -157,91 +184,141 @@ __global__ void __launch_bounds__(kThreads, RowsCfg<BN>::CTAS)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = idesc_f8(BN);
-      int it = 0;
-      for (int t = blockIdx.x; t < tiles && !*abort_flag; t += gridDim.x) {
-        for (int g = 0; g < e.groups; ++g, ++it) {
-          const int s = it % S, b = it & 1;
-          if ((it >= 2 && !mbar_wait(&pempty[b], ((it >> 1) & 1) ^ 1, abort_flag)) ||
-              !mbar_wait(&full[s], (it / S) & 1, abort_flag)) {
-            if (!*abort_flag) atomicExch(e.err, kFp8TimeoutMma);
-            *abort_flag = 1;
-            break;
-          }
-          tc::fence_after();
-          const uint32_t x0 = smem_u32(smem + size_t(s) * K::STAGE), w0 = x0 + K::TILE_X;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)  // K = 32 an instruction: 32 bytes further in the swizzled row
-            mma_f8(tmem + b * BN, tc::desc_k(x0 + k * 32), tc::desc_k(w0 + k * 32), idesc, k != 0);
-          tc::commit(&empty[s]);
-          tc::commit(&pfull[b]);
-        }
-      }
-      tc::commit(done);  // the CTA leaves (and frees its TMEM) after the last MMA
-      volatile int never = 0;
-      mbar_wait(done, 0, &never);
-    }
-  } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lanes q*32.., columns half*HN..
+    const uint32_t idesc = idesc_f8(BN);
+    const uint64_t dx0 = tc::desc_k(smem_u32(smem)), dw0 = tc::desc_k(smem_u32(smem) + K::TILE_X);
     int it = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-      const int m0 = (t % e.tiles_m) * 128, n0 = (t / e.tiles_m) * BN;
-      const int row = m0 + q * 32 + lane, c0 = n0 + half * HN;
-      const bool in = row < e.m;
-      const float* xs = e.xs + (long long)(in ? row : 0) * e.groups;
-      const float* ws = e.ws + (long long)(min(c0, e.n - 1) / kFp8Group) * e.wgroups;
-      float acc[HN];
-#pragma unroll
-      for (int j = 0; j < HN; ++j) acc[j] = 0.f;
-      float f = in ? xs[0] * ws[0] : 0.f;
-      bool ok = true;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+#pragma unroll 1
       for (int g = 0; g < e.groups; ++g, ++it) {
-        const int b = it & 1;
-        const float fn = in && g + 1 < e.groups ? xs[g + 1] * ws[g + 1] : 0.f;  // in flight beside this group
-        ok = mbar_wait(&pfull[b], (it >> 1) & 1, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) {
-          if (lane == 0 && !*abort_flag) atomicExch(e.err, kFp8TimeoutEpi);
+        const int s = it % S, b = it & 1;
+        ok = (it < 2 || mbar_wait(&pempty[b], ((it >> 1) & 1) ^ 1, abort_flag)) && mbar_wait(&full[s], (it / S) & 1, abort_flag);
+        if (!(ok = __all_sync(0xffffffffu, ok))) {
+          if (lane == 0 && !*abort_flag) atomicExch(e.err, kFp8TimeoutMma);
           *abort_flag = 1;
-          ok = false;
           break;
         }
         tc::fence_after();
+        const uint64_t dx = tc::desc_at(dx0, s * K::STAGE), dw = tc::desc_at(dw0, s * K::STAGE);
+        if (tc::elect()) {
 #pragma unroll
-        for (int j = 0; j < HN; j += 32) {
-          uint32_t r[32];
-          tc::tmem_ld32(tmem + (uint32_t(q * 32) << 16) + uint32_t(b * BN + half * HN + j), r);
+          for (int k = 0; k < 4; ++k)  // K = 32 an instruction: 32 bytes further in the swizzled row
+            mma_f8(tmem + b * BN, tc::desc_at(dx, k * 32), tc::desc_at(dw, k * 32), idesc, k != 0);
+          tc::commit(&empty[s]);
+          tc::commit(&pfull[b]);
+        }
+        __syncwarp();
+      }
+    }
+    if (tc::elect()) tc::commit(done);  // the CTA leaves (and frees its TMEM) after the last MMA
+    __syncwarp();
+    volatile int never = 0;
+    mbar_wait(done, 0, &never);
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(K::HIGH));
+    const int q = warp & 3, part = (warp - 4) >> 2;  // TMEM lanes q*32.., columns part*HN..
+    // this warp's share of a block of scales: rows 16 ew .. 16 ew + 15, two a load
+    const int ew = warp - 4, fg = lane % kXB, fr = ew * 16 + lane / kXB;
+    float fetched[8];
+    const auto fetch = [&](int t, int g0) {
+      const int m0 = (t % e.tiles_m) * 128;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = m0 + fr + 2 * i;
+        fetched[i] = r < e.m && g0 + fg < e.groups ? e.xs[(long long)r * e.groups + g0 + fg] : 0.f;
+      }
+    };
+    if (int(blockIdx.x) < tiles) fetch(blockIdx.x, 0);
+    int it = 0;
+    bool ok = true;  // false: this warp computes and stores nothing more, but keeps to the barriers
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+      const int m0 = (t % e.tiles_m) * 128, n0 = (t / e.tiles_m) * BN;
+      const int row = m0 + q * 32 + lane, c0 = n0 + part * HN;
+      const bool in = row < e.m;
+      const float* ws = e.ws + (long long)(min(c0, e.n - 1) / kFp8Group) * e.wgroups;
+      float2 acc[HN / 2];
+#pragma unroll
+      for (int j = 0; j < HN / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+      float wn = ws[0];  // the next group's scale, in flight beside this group
+#pragma unroll 1
+      for (int g = 0; g < e.groups; ++g, ++it) {
+        const int b = it & 1;
+        if (g % kXB == 0) {
+          named_bar(1, 32 * K::EPI);  // everyone has used the block before
+#pragma unroll
+          for (int i = 0; i < 8; ++i) xsm[fg * kXStride + fr + 2 * i] = fetched[i];
+          named_bar(1, 32 * K::EPI);
+          if (g + kXB < e.groups)
+            fetch(t, g + kXB);
+          else if (t + int(gridDim.x) < tiles)
+            fetch(t + gridDim.x, 0);
+        }
+        const float f = xsm[(g % kXB) * kXStride + q * 32 + lane] * wn;
+        wn = ws[min(g + 1, e.groups - 1)];
+        if (ok) {
+          ok = mbar_wait(&pfull[b], (it >> 1) & 1, abort_flag);
+          if (!(ok = __all_sync(0xffffffffu, ok))) {
+            if (lane == 0 && !*abort_flag) atomicExch(e.err, kFp8TimeoutEpi);
+            *abort_flag = 1;
+          }
+        }
+        if (!ok) continue;
+        tc::fence_after();
+        // LD columns arrive while the LD before them are added
+        constexpr int LD = BN == 256 ? 32 : 16;
+        const uint32_t at = tmem + (uint32_t(q * 32) << 16) + uint32_t(b * BN + part * HN);
+        uint32_t r[2][LD];
+        const auto load = [&](int j) {
+          if constexpr (LD == 32)
+            tc::tmem_ld32(at + j * LD, r[j & 1]);
+          else
+            tc::tmem_ld16(at + j * LD, r[j & 1]);
+        };
+        load(0);
+#pragma unroll
+        for (int j = 0; j < HN / LD; ++j) {
           tc::tmem_wait_ld();
-          tc::landed(r);
-          if (j + 32 >= HN) {  // read: the next group but one may overwrite it
+          tc::landed(r[j & 1]);
+          if (j + 1 < HN / LD) {
+            load(j + 1);
+          } else {  // read: the next group but one may overwrite it
             tc::fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&pempty[b]);
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) acc[j + i] = fmaf(__uint_as_float(r[i]), f, acc[j + i]);
-        }
-        f = fn;
-      }
-      if (!ok) break;
-      if (in) {
-        const long long at = (long long)row * e.ldy + c0;
-#pragma unroll
-        for (int j = 0; j < HN; j += 8) {
-          if (c0 + j >= e.n) break;
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[i] = acc[j + i];
-            if (e.bias && c0 + j + i < e.n) v[i] += e.bias[c0 + j + i];
-            if (e.relu) v[i] = v[i] < 0.f ? 0.f : v[i];
+          for (int i = 0; i < LD / 2; ++i) {
+            acc[j * (LD / 2) + i].x = fmaf(__uint_as_float(r[j & 1][2 * i]), f, acc[j * (LD / 2) + i].x);
+            acc[j * (LD / 2) + i].y = fmaf(__uint_as_float(r[j & 1][2 * i + 1]), f, acc[j * (LD / 2) + i].y);
           }
-          if (e.vec && c0 + j + 8 <= e.n) {
-            store8_y(e, at + j, v);
-          } else {
+        }
+      }
+      // The accumulators' registers fix the unrolling, so the stores are kept to a
+      // few instructions a column: as one general path they were 25 KB of code, and
+      // fetching it once a tile took as long as twelve groups.
+      if (ok && in) {
+        const long long at = (long long)row * e.ldy + c0;
+        if (e.vec && c0 + HN <= e.n) {
+          if (e.bias || e.relu) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (c0 + j + i < e.n) store_as(e.y_type, e.y, size_t(at + j + i), v[i]);
+            for (int j = 0; j < HN / 2; j += 2) {
+              const float4 w = e.bias ? *reinterpret_cast<const float4*>(e.bias + c0 + 2 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+              acc[j] = activate(make_float2(acc[j].x + w.x, acc[j].y + w.y), e.relu);
+              acc[j + 1] = activate(make_float2(acc[j + 1].x + w.z, acc[j + 1].y + w.w), e.relu);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < HN / 2; j += 8) store16_y<Y>(e.y, at + 2 * j, acc + j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < HN; ++j) {
+            if (c0 + j < e.n) {
+              float v = j & 1 ? acc[j / 2].y : acc[j / 2].x;
+              if (e.bias) v += e.bias[c0 + j];
+              if (e.relu) v = v < 0.f ? 0.f : v;
+              LowP<Y>::store(e.y, size_t(at + j), v);
+            }
           }
         }
       }
@@ -333,27 +410,31 @@ __global__ void __launch_bounds__(kFewThreads)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      for (int it = 0; it < ng; ++it) {
-        const int s = it % stages, b = it & 1;
-        if ((it >= 2 && !mbar_wait(&pempty[b], ((it >> 1) & 1) ^ 1, abort_flag)) ||
-            !mbar_wait(&full[s], (it / stages) & 1, abort_flag)) {
-          if (!*abort_flag) atomicExch(e.err, kFp8TimeoutMma);
-          *abort_flag = 1;
-          break;
-        }
-        tc::fence_after();
-        const uint32_t w0 = smem_u32(smem + size_t(s) * K::STAGE), x0 = w0 + K::TILE_W;
+    const uint64_t dw0 = tc::desc_k(smem_u32(smem)), dx0 = tc::desc_k(smem_u32(smem) + K::TILE_W);
+#pragma unroll 1
+    for (int it = 0; it < ng; ++it) {
+      const int s = it % stages, b = it & 1;
+      bool ok = (it < 2 || mbar_wait(&pempty[b], ((it >> 1) & 1) ^ 1, abort_flag)) && mbar_wait(&full[s], (it / stages) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) {
+        if (lane == 0 && !*abort_flag) atomicExch(e.err, kFp8TimeoutMma);
+        *abort_flag = 1;
+        break;
+      }
+      tc::fence_after();
+      const uint64_t dx = tc::desc_at(dx0, s * K::STAGE), dw = tc::desc_at(dw0, s * K::STAGE);
+      if (tc::elect()) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          mma_f8(tmem + b * BR, tc::desc_k(w0 + k * 32), tc::desc_k(x0 + k * 32), idesc_f8(BR), k != 0);
+          mma_f8(tmem + b * BR, tc::desc_at(dw, k * 32), tc::desc_at(dx, k * 32), idesc_f8(BR), k != 0);
         tc::commit(&empty[s]);
         tc::commit(&pfull[b]);
       }
-      tc::commit(done);
-      volatile int never = 0;
-      mbar_wait(done, 0, &never);
+      __syncwarp();
     }
+    if (tc::elect()) tc::commit(done);
+    __syncwarp();
+    volatile int never = 0;
+    mbar_wait(done, 0, &never);
   } else {
     const int q = warp & 3, tid = threadIdx.x - 64;
     // the scales of this CTA's rows and groups, while the first tiles arrive
@@ -423,18 +504,25 @@ __global__ void __launch_bounds__(kFewThreads)
 
 constexpr size_t kSmemMax = 227 * 1024;
 
-template <int BN>
-void launch_rows(const Fp8GemmParams& p, Args e, cudaStream_t s) {
+template <int BN, int Y>
+void launch_rows_y(const Fp8GemmParams& p, Args e, cudaStream_t s) {
   using K = RowsCfg<BN>;
   CUtensorMap tx, tw;
   tc::make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.x, p.k, p.m, p.ldx, kKB, 128);
   tc::make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.k, p.n, p.ldw, kKB, BN);
   e.tiles_m = ceil_div(p.m, 128);
   e.tiles_n = ceil_div(p.n, BN);
-  B2E_CUDA(cudaFuncSetAttribute(k_fp8_rows<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(K::SMEM)));
+  B2E_CUDA(cudaFuncSetAttribute(k_fp8_rows<BN, Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(K::SMEM)));
   const int grid = int(std::min<long long>((long long)e.tiles_m * e.tiles_n, 148LL * K::CTAS));
-  k_fp8_rows<BN><<<grid, kThreads, K::SMEM, s>>>(tx, tw, e);
+  k_fp8_rows<BN, Y><<<grid, K::THREADS, K::SMEM, s>>>(tx, tw, e);
   B2E_CUDA(cudaGetLastError());
+}
+
+template <int BN>
+void launch_rows(const Fp8GemmParams& p, const Args& e, cudaStream_t s) {
+  if (p.y_type == kF32) return launch_rows_y<BN, kF32>(p, e, s);
+  if (p.y_type == kBF16) return launch_rows_y<BN, kBF16>(p, e, s);
+  launch_rows_y<BN, kF16>(p, e, s);
 }
 
 template <int BR>
@@ -471,7 +559,7 @@ void fp8_gemm(const Fp8GemmParams& p, cudaStream_t s) {
   const int esz = int(dtype_size(p.y_type));
   Args e{p.xs, p.ws, p.bias, p.y, p.ldy, p.m, p.n, ceil_div(p.k, kFp8Group), ceil_div(p.k, kFp8Group),
          p.relu, p.y_type, 0, 0, 0, p.err};
-  e.vec = (reinterpret_cast<uintptr_t>(p.y) % (8 * esz)) == 0 && p.ldy % 8 == 0;
+  e.vec = reinterpret_cast<uintptr_t>(p.y) % 32 == 0 && (p.ldy * esz) % 32 == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
   if (p.m <= 16) return launch_few<16>(p, e, s);
   if (p.m <= 32) return launch_few<32>(p, e, s);
   if (p.m <= 64) return launch_few<64>(p, e, s);

@@ -21,35 +21,60 @@ namespace {
 // ------------------------------------------------------------ single tokens
 //
 // Bound by HBM: the state is read and written once (64 KB a head at 64 x 128)
-// and everything else is small. A CTA of eight warps takes a block of state
-// rows; eight lanes cover one state row (Q vectors of four floats each), so a
-// row's sum is three shuffles, and all loads of a thread are in flight before
-// its first use.
+// and everything else is small. A CTA of four warps takes a block of state rows:
+// LPR lanes cover one row (Q vectors of four floats each), a thread holds R
+// vectors, all in flight before their first use, and R row sums close together:
+// each exchange also halves the sums a lane carries on. Short CTAs, eight or more
+// on an SM, keep 128 KB in flight there.
 
-template <int T, int Q>
-__global__ void __launch_bounds__(256) k_scan_step(const ScanParams p, int rows_per_cta) {
-  constexpr int MAXR = 2;  // state rows a thread takes: 256 / 8 lanes = 32 a round
+// Sums of R values a lane over the LPR lanes of a row group: lane l of the group
+// ends with the sum of value `which`, complete when its other index bits are zero.
+template <int LPR, int R>
+__device__ __forceinline__ float group_sums(float (&v)[R], int lane, int& which) {
+  which = 0;
+  int n = R;
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) {
+    if (n > 1) {
+      const bool up = lane & o;
+      n >>= 1;
+#pragma unroll
+      for (int i = 0; i < R / 2; ++i)
+        if (i < n) {
+          const float send = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+      which = which * 2 + (up ? 1 : 0);
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    }
+  }
+  return v[0];
+}
+
+template <int T, int LPR, int Q, int R>
+__global__ void __launch_bounds__(128) k_scan_step(const ScanParams p) {
+  constexpr int RPW = 32 / LPR;  // rows a warp takes in one vector
   const int seq = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
   const int slot = p.plan.slots ? p.plan.slots[seq] : seq;
   if (slot < 0 || slot >= p.plan.state_rows) {
     if (threadIdx.x == 0 && p.err) *p.err = 1;
     return;
   }
-  const int c0 = threadIdx.x % 8, r0 = blockIdx.y * rows_per_cta + threadIdx.x / 8;
-  const int rend = min(p.size, (int(blockIdx.y) + 1) * rows_per_cta), nv = p.state / 4;
+  const int lane = threadIdx.x & 31, c0 = lane % LPR, nv = p.state / 4;
+  const int r0 = (blockIdx.y * 4 + (threadIdx.x >> 5)) * (R * RPW) + lane / LPR;  // rows r0 + RPW i
   float4* H = reinterpret_cast<float4*>(p.ssm + ((long long)slot * p.heads + h) * p.size * p.state);
-  float4 cur[MAXR][Q];
+  float4 cur[R][Q];
 #pragma unroll
-  for (int i = 0; i < MAXR; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int q = 0; q < Q; ++q)
-      if (r0 + 32 * i < rend && c0 + 8 * q < nv) cur[i][q] = ld_stream(H + (long long)(r0 + 32 * i) * nv + c0 + 8 * q);
+      if (r0 + RPW * i < p.size && c0 + LPR * q < nv) cur[i][q] = ld_stream(H + (long long)(r0 + RPW * i) * nv + c0 + LPR * q);
   const float dtr = p.dt[seq * p.lddt + h];
-  const float dt = p.softplus ? softplusf_(dtr) : dtr, dc = expf(p.a[h] * dt), dv = p.d ? p.d[h] : 0.f;
   float4 b[Q], c[Q];
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
-    const int n = (c0 + 8 * q) * 4;
+    const int n = (c0 + LPR * q) * 4;
     float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (n < p.state) {
 #pragma unroll
@@ -61,30 +86,36 @@ __global__ void __launch_bounds__(256) k_scan_step(const ScanParams p, int rows_
     b[q] = make_float4(t[0], t[1], t[2], t[3]);
     c[q] = make_float4(t[4], t[5], t[6], t[7]);
   }
+  const float dt = p.softplus ? softplusf_(dtr) : dtr, dc = expf(p.a[h] * dt);
+  float dot[R], xs[R];
 #pragma unroll
-  for (int i = 0; i < MAXR; ++i) {
-    const int r = r0 + 32 * i;
-    float dot = 0.f, xv = 0.f;
-    if (r < rend) {
-      xv = LowP<T>::load(p.x, size_t(seq * p.ldx + h * p.size + r));
-      const float u = dt * xv;
+  for (int i = 0; i < R; ++i)
+    xs[i] = r0 + RPW * i < p.size ? LowP<T>::load(p.x, size_t(seq * p.ldx + h * p.size + r0 + RPW * i)) : 0.f;
 #pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        if (c0 + 8 * q >= nv) continue;
-        const float4 o = cur[i][q];
-        const float4 n = make_float4(fmaf(dc, o.x, u * b[q].x), fmaf(dc, o.y, u * b[q].y), fmaf(dc, o.z, u * b[q].z),
-                                     fmaf(dc, o.w, u * b[q].w));
-        st_stream(H + (long long)r * nv + c0 + 8 * q, n);
-        dot += fmaf(c[q].w, n.w, fmaf(c[q].z, n.z, fmaf(c[q].y, n.y, c[q].x * n.x)));
-      }
+  for (int i = 0; i < R; ++i) {
+    dot[i] = 0.f;
+    const float u = dt * xs[i];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      if (r0 + RPW * i >= p.size || c0 + LPR * q >= nv) continue;
+      const float4 o = cur[i][q];
+      const float4 n = make_float4(fmaf(dc, o.x, u * b[q].x), fmaf(dc, o.y, u * b[q].y), fmaf(dc, o.z, u * b[q].z),
+                                   fmaf(dc, o.w, u * b[q].w));
+      st_stream(H + (long long)(r0 + RPW * i) * nv + c0 + LPR * q, n);
+      dot[i] += fmaf(c[q].w, n.w, fmaf(c[q].z, n.z, fmaf(c[q].y, n.y, c[q].x * n.x)));
     }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (r < rend && c0 == 0) {
-      float y = fmaf(dv, xv, dot);
-      if (p.z) y *= siluf_(LowP<T>::load(p.z, size_t(seq * p.ldz + h * p.size + r)));
-      LowP<T>::store(p.y, size_t(seq * p.ldy + h * p.size + r), y);
-    }
+  }
+  int which;
+  const float sum = group_sums<LPR, R>(dot, lane, which);
+  // every lane of a row group holds one of its rows' sums; the lanes that hold
+  // the same one differ in the bits behind those that chose it
+  constexpr int TAIL = LPR > R ? LPR / R : 1;
+  const int r = r0 + RPW * which;
+  if (r < p.size && c0 % TAIL == 0) {
+    const float dv = p.d ? p.d[h] : 0.f;
+    float y = fmaf(dv, LowP<T>::load(p.x, size_t(seq * p.ldx + h * p.size + r)), sum);
+    if (p.z) y *= siluf_(LowP<T>::load(p.z, size_t(seq * p.ldz + h * p.size + r)));
+    LowP<T>::store(p.y, size_t(seq * p.ldy + h * p.size + r), y);
   }
 }
 
@@ -324,15 +355,16 @@ void launch_step(const ScanParams& p, cudaStream_t s) {
   if (p.state % 4 != 0) {
     k_scan_step_any<T><<<unsigned(items), 256, 0, s>>>(p);
   } else {
-    // blocks of 64 state rows; 32 where there are few heads to spread over the SMs
-    const int rows = items * ceil_div(p.size, 64) >= 148 * 2 ? 64 : 32;
-    const dim3 grid{unsigned(items), unsigned(ceil_div(p.size, rows)), 1};
-    if (p.state <= 64)
-      k_scan_step<T, 2><<<grid, 256, 0, s>>>(p, rows);
+    // lanes of a row by its width; rows a CTA takes: 4 warps x R vectors x 32 / LPR
+    const auto grid = [&](int rows) { return dim3{unsigned(items), unsigned(ceil_div(p.size, rows)), 1}; };
+    if (p.state <= 32)
+      k_scan_step<T, 8, 1, 8><<<grid(128), 128, 0, s>>>(p);
+    else if (p.state <= 64)
+      k_scan_step<T, 16, 1, 8><<<grid(64), 128, 0, s>>>(p);
     else if (p.state <= 128)
-      k_scan_step<T, 4><<<grid, 256, 0, s>>>(p, rows);
+      k_scan_step<T, 32, 1, 8><<<grid(32), 128, 0, s>>>(p);
     else
-      k_scan_step<T, 8><<<grid, 256, 0, s>>>(p, rows);
+      k_scan_step<T, 32, 2, 4><<<grid(16), 128, 0, s>>>(p);
   }
   B2E_CUDA(cudaGetLastError());
 }

@@ -216,11 +216,14 @@ class NormFp8(NamedTuple):
 def _call(name: str, device, *args) -> None:
     """One C-ABI call on `device`'s current stream."""
     fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == device.index:
-        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc)
 
 
 def _at(t) -> Optional[int]:
