@@ -5,13 +5,15 @@
 //   v = window[slot] ++ x[sequence];  y[t] = act(bias + sum_j w[j] v[t + j]);  window[slot] <- last taps - 1 of v
 //
 // Bound by HBM: each x and y once, a window once each way. A warp takes 32
-// vectors of four channels over a tile of tokens and keeps the
+// vectors of channels (16 bytes of x a lane) over a tile of tokens and keeps the
 // last taps - 1 inputs in registers, so a token is read once and a tile reads
-// only taps - 1 inputs of its neighbour's again. The tile that starts a
-// sequence is the only one that reads the window, and it writes it too: no
-// other tile can see the new one.
+// only taps - 1 inputs of its neighbour's again; the next few tokens are in flight
+// while one batch is computed, channels in packed pairs. The tile that starts a
+// sequence is the only one that reads the window, and it writes it too: no other
+// tile can see the new one.
 #include <algorithm>
 
+#include "packed.cuh"
 #include "seqops.cuh"
 
 namespace b2e {
@@ -19,56 +21,67 @@ namespace {
 
 constexpr int kConvWarps = 4;
 
+// VC channels of a token as they lie in memory, two values a register in 16 bits.
 template <int T, int VC>
-__device__ __forceinline__ void load_vec(const void* p, long long i, float (&v)[VC]) {
-  if constexpr (VC == 1) {
-    v[0] = LowP<T>::load(p, size_t(i));
-  } else if constexpr (T == kF32) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i));
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  } else {
-    const uint2 r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + i));
-    const uint32_t u[2] = {r.x, r.y};
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if constexpr (T == kBF16) {
-        v[2 * j] = __uint_as_float(u[j] << 16);
-        v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
-        v[2 * j] = f.x;
-        v[2 * j + 1] = f.y;
-      }
+struct Raw {
+  static constexpr int N = T == kF32 || VC == 1 ? VC : VC / 2;
+  uint32_t u[N];
+  __device__ __forceinline__ void load(const void* p) {
+    if constexpr (VC == 1 && T != kF32) {
+      u[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+    } else if constexpr (N == 4) {
+      const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
+      u[0] = r.x; u[1] = r.y; u[2] = r.z; u[3] = r.w;
+    } else if constexpr (N == 2) {
+      const uint2 r = __ldg(reinterpret_cast<const uint2*>(p));
+      u[0] = r.x; u[1] = r.y;
+    } else {
+      u[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
     }
   }
-}
+  __device__ __forceinline__ F2 pair(int i) const {
+    if constexpr (T == kF32) {
+      return f2(u[VC == 1 ? 0 : 2 * i], u[VC == 1 ? 0 : 2 * i + 1]);
+    } else if constexpr (T == kBF16) {
+      return f2(bf_lo(u[i]), bf_hi(u[i]));
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      return f2(f.x, f.y);
+    }
+  }
+};
 
 template <int T, int VC>
-__device__ __forceinline__ void store_vec(void* p, long long i, const float (&v)[VC]) {
-  if constexpr (VC == 1) {
-    LowP<T>::store(p, size_t(i), v[0]);
-  } else if constexpr (T == kF32) {
-    __stcs(reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i), make_float4(v[0], v[1], v[2], v[3]));
-  } else {
-    uint32_t u[2];
+__device__ __forceinline__ void store_pairs(void* p, const F2* y) {
+  float v[VC == 1 ? 2 : VC];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+  for (int i = 0; i < (VC == 1 ? 1 : VC / 2); ++i) split(y[i], v[2 * i], v[2 * i + 1]);
+  if constexpr (VC == 1) {
+    LowP<T>::store(p, 0, v[0]);
+  } else if constexpr (T == kF32) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+  } else {
+    uint32_t u[VC / 2];
+#pragma unroll
+    for (int j = 0; j < VC / 2; ++j) {
       if constexpr (T == kBF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-        u[j] = *reinterpret_cast<const uint32_t*>(&h);
+        u[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
       } else {
         const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
         u[j] = *reinterpret_cast<const uint32_t*>(&h);
       }
     }
-    __stcs(reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i), make_uint2(u[0], u[1]));
+    if constexpr (VC == 8)
+      __stcs(reinterpret_cast<uint4*>(p), make_uint4(u[0], u[1], u[2], u[3]));
+    else
+      __stcs(reinterpret_cast<uint2*>(p), make_uint2(u[0], u[1]));
   }
 }
 
 // VC * N contiguous floats, 16-byte aligned when VC > 1.
 template <int VC, int N>
 __device__ __forceinline__ void load_rows(const float* p, float (&v)[VC][N]) {
-  if constexpr (VC * N % 4 == 0 && VC > 1) {
+  if constexpr (VC > 1) {
     float flat[VC * N];
 #pragma unroll
     for (int i = 0; i < VC * N / 4; ++i) {
@@ -79,12 +92,12 @@ __device__ __forceinline__ void load_rows(const float* p, float (&v)[VC][N]) {
     for (int i = 0; i < VC * N; ++i) v[i / N][i % N] = flat[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < VC * N; ++i) v[i / N][i % N] = p[i];
+    for (int i = 0; i < N; ++i) v[0][i] = p[i];
   }
 }
 template <int VC, int N>
 __device__ __forceinline__ void store_rows(float* p, const float (&v)[VC][N]) {
-  if constexpr (VC * N % 4 == 0 && VC > 1) {
+  if constexpr (VC > 1) {
 #pragma unroll
     for (int i = 0; i < VC * N / 4; ++i)
       reinterpret_cast<float4*>(p)[i] =
@@ -92,18 +105,52 @@ __device__ __forceinline__ void store_rows(float* p, const float (&v)[VC][N]) {
                       v[(4 * i + 3) / N][(4 * i + 3) % N]);
   } else {
 #pragma unroll
-    for (int i = 0; i < VC * N; ++i) p[i] = v[i / N][i % N];
+    for (int i = 0; i < N; ++i) p[i] = v[0][i];
   }
 }
 
-// silu with the hardware's exponential and reciprocal: a relative error of a few
-// 2^-22 where the result matters, against ~40 instructions a value for the
-// library's, which would bound the kernel ahead of HBM.
-__device__ __forceinline__ float silu_fast(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
+// Column j of a window (or of the weights) in pairs of channels.
+template <int VC, int N>
+__device__ __forceinline__ F2 pair_of(const float (&v)[VC][N], int i, int j) {
+  return VC == 1 ? f2(v[0][j], v[0][j]) : f2(v[2 * i % VC][j], v[(2 * i + 1) % VC][j]);
+}
+
+template <int VC, int TAPS>
+struct Weights {
+  static constexpr int P = VC == 1 ? 1 : VC / 2, W = TAPS - 1;
+  F2 w[TAPS][P], bias[P];
+  __device__ __forceinline__ Weights(const float* weight, const float* b) {
+    float v[VC][TAPS];
+    load_rows<VC, TAPS>(weight, v);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+#pragma unroll
+      for (int j = 0; j < TAPS; ++j) w[j][i] = pair_of(v, i, j);
+      bias[i] = b ? f2(b[VC == 1 ? 0 : 2 * i], b[VC == 1 ? 0 : 2 * i + 1]) : f2(0.f, 0.f);
+    }
+  }
+  // One token: `last` are the inputs before it, which move on by one.
+  template <int T>
+  __device__ __forceinline__ void token(F2 (&last)[W][P], const Raw<T, VC>& raw, int silu, F2 (&y)[P]) const {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const F2 in = raw.pair(i);
+      y[i] = bias[i];
+#pragma unroll
+      for (int j = 0; j < W; ++j) y[i] = fma2(w[j][i], last[j][i], y[i]);
+      y[i] = fma2(w[W][i], in, y[i]);
+      if (silu) y[i] = silu2(y[i]);
+#pragma unroll
+      for (int j = 0; j + 1 < W; ++j) last[j][i] = last[j + 1][i];
+      last[W - 1][i] = in;
+    }
+  }
+};
 
 template <int T, int VC, int TAPS>
 __global__ void __launch_bounds__(32 * kConvWarps) k_conv(const ConvParams p, int len, int vblocks, long long warps) {
-  constexpr int W = TAPS - 1, U = 8;  // tokens whose loads are in flight together
+  constexpr int W = TAPS - 1, P = VC == 1 ? 1 : VC / 2, U = VC == 8 ? 4 : 8;  // U tokens in flight
+  constexpr int ESZ = T == kF32 ? 4 : 2;
   const long long gw = (long long)blockIdx.x * kConvWarps + (threadIdx.x >> 5);
   if (gw >= warps) return;
   const int tile = int(gw / vblocks), lane = threadIdx.x & 31;
@@ -116,71 +163,80 @@ __global__ void __launch_bounds__(32 * kConvWarps) k_conv(const ConvParams p, in
     if (p.err) *p.err = 1;
     return;
   }
-  float w[VC][TAPS], bias[VC];
-  load_rows<VC, TAPS>(p.w + (long long)c * TAPS, w);
-#pragma unroll
-  for (int i = 0; i < VC; ++i) bias[i] = p.bias ? p.bias[c + i] : 0.f;
-  float* win = p.window + ((long long)slot * p.channels + c) * W;
+  const int end = min(t.end, t.first + len);
   const bool head = t.first == t.start;
-  float last[W][VC], old[VC][W];  // last[j]: input of token first - W + j
+  const long long xs = p.ldx * ESZ, ys = p.ldy * ESZ;
+  const char* xp = reinterpret_cast<const char*>(p.x) + t.first * xs + (long long)c * ESZ;
+  char* yp = reinterpret_cast<char*>(p.y) + t.first * ys + (long long)c * ESZ;
+  int left = end - t.first;
+  Raw<T, VC> raw[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (u < left) raw[u].load(xp + u * xs);
+  const Weights<VC, TAPS> k(p.w + (long long)c * TAPS, p.bias ? p.bias + c : nullptr);
+  float* win = p.window + ((long long)slot * p.channels + c) * W;
+  F2 last[W][P];  // last[j]: input of token first - W + j
   if (head) {
+    float old[VC][W], neu[VC][W];
     load_rows<VC, W>(win, old);
 #pragma unroll
     for (int j = 0; j < W; ++j)
 #pragma unroll
-      for (int i = 0; i < VC; ++i) last[j][i] = old[i][j];
-  } else {  // a tile holds more than W tokens: the inputs before a later tile are the sequence's
-#pragma unroll
-    for (int j = 0; j < W; ++j) load_vec<T, VC>(p.x, (t.first - W + j) * p.ldx + c, last[j]);
-  }
-  const int end = min(t.end, t.first + len);
-  for (int t0 = t.first; t0 < end; t0 += U) {
-    float in[U][VC];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (t0 + u < end) load_vec<T, VC>(p.x, (t0 + u) * p.ldx + c, in[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (t0 + u < end) {
-        float y[VC];
-#pragma unroll
-        for (int i = 0; i < VC; ++i) {
-          float s = bias[i];
-#pragma unroll
-          for (int j = 0; j < W; ++j) s = fmaf(w[i][j], last[j][i], s);
-          s = fmaf(w[i][W], in[u][i], s);
-          y[i] = p.silu ? silu_fast(s) : s;
-#pragma unroll
-          for (int j = 0; j + 1 < W; ++j) last[j][i] = last[j + 1][i];
-          last[W - 1][i] = in[u][i];
-        }
-        store_vec<T, VC>(p.y, (t0 + u) * p.ldy + c, y);
-      }
-    }
-  }
-  if (head) {
+      for (int i = 0; i < P; ++i) last[j][i] = pair_of(old, i, j);
     const int n = t.end - t.start;
-    float neu[VC][W];
 #pragma unroll
     for (int j = 0; j < W; ++j) {
       const int at = n - W + j;  // token of the sequence, or at + W of the old window
-      if (at >= 0) {
-        float in[VC];
-        load_vec<T, VC>(p.x, (t.start + at) * p.ldx + c, in);
+      Raw<T, VC> in;
+      if (at >= 0) in.load(xp + at * xs);
 #pragma unroll
-        for (int i = 0; i < VC; ++i) neu[i][j] = in[i];
-      } else {
+      for (int i = 0; i < P; ++i) {
+        float a = 0.f, b = 0.f;
+        if (at >= 0) {
+          split(in.pair(i), a, b);
+        } else {
 #pragma unroll
-        for (int i = 0; i < VC; ++i) {
-          neu[i][j] = 0.f;
-#pragma unroll
-          for (int k = 0; k < W; ++k)
-            if (k == at + W) neu[i][j] = old[i][k];
+          for (int o = 0; o < W; ++o)
+            if (o == at + W) split(pair_of(old, i, o), a, b);
         }
+        neu[VC == 1 ? 0 : 2 * i][j] = a;
+        if (VC > 1) neu[(2 * i + 1) % VC][j] = b;
       }
     }
     store_rows<VC, W>(win, neu);
+  } else {  // a tile holds more than W tokens: the inputs before a later tile are the sequence's
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      Raw<T, VC> in;
+      in.load(xp - (W - j) * xs);
+#pragma unroll
+      for (int i = 0; i < P; ++i) last[j][i] = in.pair(i);
+    }
   }
+  F2 y[P];
+#pragma unroll 1
+  for (; left >= U; left -= U) {
+    xp += U * xs;
+    Raw<T, VC> next[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < left - U) next[u].load(xp + u * xs);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      k.token(last, raw[u], p.silu, y);
+      store_pairs<T, VC>(yp, y);
+      yp += ys;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = next[u];
+  }
+#pragma unroll
+  for (int u = 0; u < U - 1; ++u)
+    if (u < left) {
+      k.token(last, raw[u], p.silu, y);
+      store_pairs<T, VC>(yp, y);
+      yp += ys;
+    }
 }
 
 // One token a sequence: the windows' bytes count. A warp takes kStepSeqs
@@ -190,11 +246,12 @@ constexpr int kStepSeqs = 4;
 
 template <int T, int VC, int TAPS>
 __global__ void __launch_bounds__(32 * kConvWarps) k_conv_step(const ConvParams p, int vblocks, long long warps) {
-  constexpr int W = TAPS - 1;
+  constexpr int W = TAPS - 1, P = VC == 1 ? 1 : VC / 2, ESZ = T == kF32 ? 4 : 2;
   const long long gw = (long long)blockIdx.x * kConvWarps + (threadIdx.x >> 5);
   const int c = (int(gw % vblocks) * 32 + int(threadIdx.x & 31)) * VC, s0 = int(gw / vblocks) * kStepSeqs;
   if (gw >= warps || c >= p.channels) return;
-  float old[kStepSeqs][VC][W], in[kStepSeqs][VC];
+  float old[kStepSeqs][VC][W];
+  Raw<T, VC> in[kStepSeqs];
   long long at[kStepSeqs];
 #pragma unroll
   for (int i = 0; i < kStepSeqs; ++i) {
@@ -210,78 +267,77 @@ __global__ void __launch_bounds__(32 * kConvWarps) k_conv_step(const ConvParams 
     at[i] = slot < 0 ? -1 : ((long long)slot * p.channels + c) * W;
     if (slot >= 0) {
       load_rows<VC, W>(p.window + at[i], old[i]);
-      load_vec<T, VC>(p.x, s * p.ldx + c, in[i]);
+      in[i].load(reinterpret_cast<const char*>(p.x) + (s * p.ldx + c) * ESZ);
     }
   }
-  float w[VC][TAPS], bias[VC];
-  load_rows<VC, TAPS>(p.w + (long long)c * TAPS, w);
-#pragma unroll
-  for (int i = 0; i < VC; ++i) bias[i] = p.bias ? p.bias[c + i] : 0.f;
+  const Weights<VC, TAPS> k(p.w + (long long)c * TAPS, p.bias ? p.bias + c : nullptr);
 #pragma unroll
   for (int i = 0; i < kStepSeqs; ++i) {
     if (at[i] < 0) continue;
-    float y[VC];
+    F2 last[W][P], y[P];
 #pragma unroll
-    for (int k = 0; k < VC; ++k) {
-      float s = bias[k];
+    for (int j = 0; j < W; ++j)
 #pragma unroll
-      for (int j = 0; j < W; ++j) s = fmaf(w[k][j], old[i][k][j], s);
-      s = fmaf(w[k][W], in[i][k], s);
-      y[k] = p.silu ? silu_fast(s) : s;
+      for (int n = 0; n < P; ++n) last[j][n] = pair_of(old[i], n, j);
+    k.token(last, in[i], p.silu, y);
+    store_pairs<T, VC>(reinterpret_cast<char*>(p.y) + ((s0 + i) * p.ldy + c) * ESZ, y);
 #pragma unroll
-      for (int j = 0; j + 1 < W; ++j) old[i][k][j] = old[i][k][j + 1];
-      old[i][k][W - 1] = in[i][k];
-    }
-    store_vec<T, VC>(p.y, (s0 + i) * p.ldy + c, y);
+    for (int j = 0; j < W; ++j)
+#pragma unroll
+      for (int n = 0; n < P; ++n) {
+        float a, b;
+        split(last[j][n], a, b);
+        old[i][VC == 1 ? 0 : 2 * n][j] = a;
+        if (VC > 1) old[i][(2 * n + 1) % VC][j] = b;
+      }
     store_rows<VC, W>(p.window + at[i], old[i]);
   }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-template <int T, int VC, int TAPS>
+template <int T, int VC, int TAPS, bool step>
 void launch(const ConvParams& p, cudaStream_t s) {
   const int vblocks = ceil_div(p.channels, 32 * VC);
-  const bool step = p.plan.starts == nullptr;
   // Tiles of 32 tokens read 3 of them again; short tiles where long ones would
   // leave the SMs without enough loads in flight.
   const int len = (long long)p.plan.tokens * vblocks >= 32LL * 148 * 16 ? 32 : 8;
   const long long warps = (step ? ceil_div(p.plan.seqs, kStepSeqs) : seq_tiles(p.plan, len)) * vblocks;
   const long long grid = (warps + kConvWarps - 1) / kConvWarps;
   B2E_CHECK(grid <= 0x7fffffffLL, kErrInvalid, "causal_conv: too many tiles");
-  if (step)
+  if constexpr (step)
     k_conv_step<T, VC, TAPS><<<unsigned(grid), 32 * kConvWarps, 0, s>>>(p, vblocks, warps);
   else
     k_conv<T, VC, TAPS><<<unsigned(grid), 32 * kConvWarps, 0, s>>>(p, len, vblocks, warps);
   B2E_CUDA(cudaGetLastError());
 }
 
-template <int T, int VC>
+template <int T, int VC, bool step>
 void launch_taps(const ConvParams& p, cudaStream_t s) {
-  if (p.taps == 2) return launch<T, VC, 2>(p, s);
-  if (p.taps == 3) return launch<T, VC, 3>(p, s);
-  launch<T, VC, 4>(p, s);
+  if (p.taps == 2) return launch<T, VC, 2, step>(p, s);
+  if (p.taps == 3) return launch<T, VC, 3, step>(p, s);
+  launch<T, VC, 4, step>(p, s);
 }
 
-template <int T>
+template <int T, bool step>
 void launch_type(const ConvParams& p, cudaStream_t s) {
-  constexpr int VC = 4;
-  const auto aligned = [](const void* v) { return (reinterpret_cast<uintptr_t>(v) & (VC * (T == kF32 ? 4 : 2) - 1)) == 0; };
-  const bool vec = p.channels % VC == 0 && p.ldx % VC == 0 && p.ldy % VC == 0 && aligned(p.x) && aligned(p.y) &&
-                   aligned16(p.w) && aligned16(p.window);
+  constexpr int VC = T == kF32 || step ? 4 : 8;  // 16 bytes of x a lane; four channels of the windows, which bound a step
+  const auto aligned = [](const void* v, size_t a) { return (reinterpret_cast<uintptr_t>(v) & (a - 1)) == 0; };
+  const size_t xa = VC * (T == kF32 ? 4 : 2);
+  const bool vec = p.channels % VC == 0 && p.ldx % VC == 0 && p.ldy % VC == 0 && aligned(p.x, xa) && aligned(p.y, xa) &&
+                   aligned(p.w, 16) && aligned(p.window, 16);
   if (vec)
-    launch_taps<T, VC>(p, s);
+    launch_taps<T, VC, step>(p, s);
   else
-    launch_taps<T, 1>(p, s);
+    launch_taps<T, 1, step>(p, s);
 }
 
 }  // namespace
 
 void causal_conv(const ConvParams& p, cudaStream_t s) {
   if (p.plan.seqs == 0 || p.plan.tokens == 0) return;
-  if (p.type == kF32) return launch_type<kF32>(p, s);
-  if (p.type == kBF16) return launch_type<kBF16>(p, s);
-  launch_type<kF16>(p, s);
+  const bool step = p.plan.starts == nullptr;
+  if (p.type == kF32) return step ? launch_type<kF32, true>(p, s) : launch_type<kF32, false>(p, s);
+  if (p.type == kBF16) return step ? launch_type<kBF16, true>(p, s) : launch_type<kBF16, false>(p, s);
+  step ? launch_type<kF16, true>(p, s) : launch_type<kF16, false>(p, s);
 }
 
 }  // namespace b2e

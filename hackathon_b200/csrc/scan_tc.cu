@@ -37,6 +37,7 @@
 // 6 x 128 x 128 x 128 products a chunk and pair.
 #include <algorithm>
 
+#include "packed.cuh"
 #include "scan.cuh"
 #include "tc.cuh"
 
@@ -83,54 +84,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(acc));
 }
-
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-// Two float32 lanes in one instruction, each rounded as the scalar one.
-struct F2 {
-  unsigned long long v;
-};
-__device__ __forceinline__ F2 f2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ F2 f2(uint32_t a, uint32_t b) { return f2(__uint_as_float(a), __uint_as_float(b)); }
-__device__ __forceinline__ void split(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_bf16(F2 a) {
-  float x, y;
-  split(a, x, y);
-  return pack_bf16(x, y);
-}
-__device__ __forceinline__ float rcp(float x) {
-  float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
 // A sum kept as hi + lo.
 struct Pair {
@@ -571,7 +524,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const long long hp = 64LL * N;
     float* own = p.ssm + ((long long)slot * p.heads + head) * hp + (long long)pr * N;
     float* part = g.wk.state + ((long long)tile * p.heads + head) * hp + (long long)pr * N;
-    const float* from = g.seg > 0 ? part : own;
+    const float* from = g.seg > 0 && t.end - t.start > g.seg ? part : own;
     uint8_t* hrow = smem + K::oH + prow * 128;
     bool ok = true;
 #pragma unroll 1
@@ -717,7 +670,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int q = warp & 3, row = q * 32 + lane, h = (warp - 20) >> 2, head = h0 + h;
     const bool has = head < p.heads;
     const float d = has && p.d ? p.d[head] : 0.f;
-    const F2 d2 = f2(d, d), l2e = f2(-1.4426950408889634f, -1.4426950408889634f), one = f2(1.f, 1.f);
+    const F2 d2 = f2(d, d);
     const uint32_t ycol = tmem + lanes + cY + h * 64;
     bool ok = true;
 #pragma unroll 1
@@ -780,13 +733,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           F2 y = f2(r[2 * k], r[2 * k + 1]);
-          if (p.z) {  // y z / (1 + exp(-z))
-            const F2 zz = f2(bf_lo(z[k]), bf_hi(z[k]));
-            float e0, e1;
-            split(mul2(zz, l2e), e0, e1);
-            split(add2(f2(ex2(e0), ex2(e1)), one), e0, e1);
-            y = mul2(y, mul2(zz, f2(rcp(e0), rcp(e1))));
-          }
+          if (p.z) y = mul2(y, silu2(f2(bf_lo(z[k]), bf_hi(z[k]))));
           o[k] = pack_bf16(y);
         }
 #pragma unroll
