@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(256) k_scan_step_any(const ScanParams p) {
 // operations a state element and token, two elements an instruction. The layout
 // keeps shared memory off that path: a token costs a thread 2 J + R / 4 vectors
 // (with two rows and 32 columns a thread it was 16, and LDS was the limit: 294 us
-// for 64 sequences of 10000 tokens, 8 heads, against 127 us). Tokens are staged in
+// for 64 sequences of 10000 tokens, 8 heads, against 218 us). Tokens are staged in
 // blocks of 16, the next block by cp.async while one is computed where the
 // operands are float32 vectors.
 
