@@ -50,6 +50,20 @@ constexpr int kXSlots = 3;
 constexpr int kTcThreads = 896;
 constexpr int kVecs = 3;                     // chunks whose decays are held
 enum ScanError : int { kScanTimeout = 131 };
+// Registers by warpgroup, out of the launch's 28 warps x 72. The shared memory
+// leaves almost no L1, so that a spilled register is a trip to L2: with 72 for
+// everyone the y warps spilled and a chunk took three times as long.
+constexpr int kRegLaunch = 72, kRegMisc = 72, kRegS = 56, kRegX = 72, kRegY = 88;
+static_assert(4 * kRegMisc + 8 * kRegS + 8 * kRegX + 8 * kRegY <= 28 * kRegLaunch, "register shares exceed the launch's");
+template <bool ENDS, int N>
+__device__ __forceinline__ void shares() {
+  if constexpr (!ENDS) {
+    if constexpr (N < kRegLaunch)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+    else if constexpr (N > kRegLaunch)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+  }
+}
 
 // TMEM columns (of 512): G, and S of both heads in its place (each 16 columns of
 // G become 8 of either head's S in bf16 pairs); the buffers of the state's
@@ -96,11 +110,21 @@ __device__ __forceinline__ Pair add(Pair a, Pair b) {
   return {h, e - (h - s)};
 }
 __device__ __forceinline__ float diff(Pair a, Pair b) { return (a.hi - b.hi) + (a.lo - b.lo); }
-__device__ __forceinline__ Pair shfl_up(Pair a, int d) {
-  return {__shfl_up_sync(0xffffffffu, a.hi, d), __shfl_up_sync(0xffffffffu, a.lo, d)};
-}
-__device__ __forceinline__ Pair shfl(Pair a, int src) {
-  return {__shfl_sync(0xffffffffu, a.hi, src), __shfl_sync(0xffffffffu, a.lo, src)};
+// log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|), with log1p(e) = 2 atanh(s),
+// s = e / (2 + e) <= 1 / 3, by its series to s^17 (the next term is below 2^-31 of
+// the first): relative accuracy for any x, in a third of the library's instructions.
+__device__ __forceinline__ float softplus_fast(float x) {
+  const float e = ex2(fabsf(x) * -1.4426950408889634f), s = e * rcp(2.0f + e), q = s * s;
+  float r = 2.0f / 17.0f;
+  r = fmaf(r, q, 2.0f / 15.0f);
+  r = fmaf(r, q, 2.0f / 13.0f);
+  r = fmaf(r, q, 2.0f / 11.0f);
+  r = fmaf(r, q, 2.0f / 9.0f);
+  r = fmaf(r, q, 2.0f / 7.0f);
+  r = fmaf(r, q, 2.0f / 5.0f);
+  r = fmaf(r, q, 2.0f / 3.0f);
+  r = fmaf(r, q, 2.0f);
+  return fmaf(s, r, x < 0.f ? 0.f : x);
 }
 
 // Decays of one head and chunk; c in powers of two.
@@ -231,6 +255,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (lane == 0) mbar_arrive(b);
   };
 
+  if (warp < 4) {
+    shares<ENDS, kRegMisc>();
   if (warp == 0) {
     // ---- loads
     if (lane == 0) {
@@ -362,73 +388,72 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!ok && lane == 0) failed();
     }
   } else if (warp == 2) {
-    // ---- decays of both heads, four tokens a lane
+    // ---- decays: a half-warp a head, eight tokens a lane
+    const int hh = lane >> 4, l = lane & 15;
+    const bool has = h0 + hh < p.heads;
+    const float a2 = has ? p.a[h0 + hh] * 1.4426950408889634f : 0.f;
+    const float* at = p.dt + (long long)(t.first + 8 * l) * p.lddt + h0 + hh;
+    float dt[8];
+    const auto fetch = [&](int left) {  // dt of the chunk at `at`, `left` tokens
+#pragma unroll
+      for (int k = 0; k < 8; ++k) dt[k] = has && 8 * l + k < left ? at[k * p.lddt] : 0.f;
+    };
+    fetch(end - t.first);
     bool ok = true;
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
       const int st = c & 1, vs = c % kVecs, valid = min(Q, end - t.first - c * Q);
+      Pair cum[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const bool in = has && 8 * l + k < valid;
+        if (p.softplus) dt[k] = softplus_fast(dt[k]);
+        dt[k] = in ? dt[k] : 0.f;
+        // Below 2^-200 a decay is zero in float32 whatever it multiplies; the
+        // bound keeps the sums small (and keeps a NaN).
+        float x = in ? a2 * dt[k] : 0.f;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(-200.f));
+        cum[k] = k ? add(cum[k - 1], {x, 0.f}) : Pair{x, 0.f};
+      }
+      Pair sum = cum[7];
+#pragma unroll 1
+      for (int o = 1; o < 16; o <<= 1) {
+        const Pair x = {__shfl_up_sync(0xffffffffu, sum.hi, o, 16), __shfl_up_sync(0xffffffffu, sum.lo, o, 16)};
+        if (l >= o) sum = add(x, sum);
+      }
+      Pair before = {__shfl_up_sync(0xffffffffu, sum.hi, 1, 16), __shfl_up_sync(0xffffffffu, sum.lo, 1, 16)};
+      if (l == 0) before = {0.f, 0.f};
+      const auto upto = [&](int src) { return Pair{__shfl_sync(0xffffffffu, sum.hi, src, 16), __shfl_sync(0xffffffffu, sum.lo, src, 16)}; };
+      const Pair b1 = upto(3), b2 = upto(7), b3 = upto(11), total = upto(15);
+      const int blk = l >> 2;
+      const Pair base = blk == 0 ? Pair{0.f, 0.f} : blk == 1 ? b1 : blk == 2 ? b2 : b3;
       if (c >= kVecs && !(ok = wait(&vempty[vs], ((c / kVecs) & 1) ^ 1))) break;
-#pragma unroll 1
-      for (int hh = 0; hh < 2; ++hh) {
-        Vec& v = vec[vs * 2 + hh];
-        const bool has = h0 + hh < p.heads;
-        const float a2 = has ? p.a[h0 + hh] * 1.4426950408889634f : 0.f;
-        const float* at = p.dt + (long long)(t.first + c * Q + 4 * lane) * p.lddt + h0 + hh;
-        float dt[4];
+      Vec& v = vec[vs * 2 + hh];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) dt[k] = has && 4 * lane + k < valid ? at[k * p.lddt] : 0.f;
-        if (p.softplus) {
-#pragma unroll 1
-          for (int k = 0; k < 4; ++k) {  // in turn, through the first place
-            const float x = softplusf_(dt[0]);
-            dt[0] = dt[1];
-            dt[1] = dt[2];
-            dt[2] = dt[3];
-            dt[3] = x;
-          }
-        }
-        Pair cum[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool in = has && 4 * lane + k < valid;
-          dt[k] = in ? dt[k] : 0.f;
-          // Below 2^-200 a decay is zero in float32 whatever it multiplies; the
-          // bound keeps the sums small (and keeps a NaN).
-          float x = in ? a2 * dt[k] : 0.f;
-          asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(-200.f));
-          cum[k] = k ? add(cum[k - 1], {x, 0.f}) : Pair{x, 0.f};
-        }
-        Pair sum = cum[3];
-#pragma unroll 1
-        for (int o = 1; o < 32; o <<= 1) {
-          const Pair x = shfl_up(sum, o);
-          if (lane >= o) sum = add(x, sum);
-        }
-        Pair before = shfl_up(sum, 1);
-        if (lane == 0) before = {0.f, 0.f};
-        const Pair total = shfl(sum, 31), b1 = shfl(sum, 7), b2 = shfl(sum, 15), b3 = shfl(sum, 23);
-        const int blk = lane >> 3;
-        const Pair base = blk == 0 ? Pair{0.f, 0.f} : blk == 1 ? b1 : blk == 2 ? b2 : b3;
+      for (int k0 = 0; k0 < 8; k0 += 4) {
         float o[5][4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const Pair x = add(before, cum[k]);
+          const Pair x = add(before, cum[k0 + k]);
+          const float d = dt[k0 + k];
           o[0][k] = diff(base, x);
-          o[1][k] = ex2(diff(total, x)) * dt[k];
-          o[2][k] = ex2(diff(b1, x)) * dt[k];
-          o[3][k] = ex2(diff(b2, x)) * dt[k];
-          o[4][k] = ex2(diff(b3, x)) * dt[k];
+          o[1][k] = ex2(diff(total, x)) * d;
+          o[2][k] = ex2(diff(b1, x)) * d;
+          o[3][k] = ex2(diff(b2, x)) * d;
+          o[4][k] = ex2(diff(b3, x)) * d;
         }
-        auto put = [&](float* to, const float (&f)[4]) { reinterpret_cast<float4*>(to)[lane] = make_float4(f[0], f[1], f[2], f[3]); };
+        const auto put = [&](float* to, const float* f) { *reinterpret_cast<float4*>(to + 8 * l + k0) = make_float4(f[0], f[1], f[2], f[3]); };
         put(v.neg, o[0]);
-        put(v.dt, dt);
+        put(v.dt, dt + k0);
         put(v.w, o[1]);
         if (blk < 1) put(v.col, o[2]);
         if (blk < 2) put(v.col + 32, o[3]);
         if (blk < 3) put(v.col + 96, o[4]);
-        if ((lane & 7) == 0) v.base[blk] = base.hi + base.lo;
-        if (lane == 0) v.total = ex2(total.hi + total.lo);
       }
+      if ((l & 3) == 0) v.base[blk] = base.hi + base.lo;
+      if (l == 0) v.total = ex2(total.hi + total.lo);
+      at += Q * p.lddt;
+      fetch(end - t.first - (c + 1) * Q);
       if (valid < Q) {
         // Behind the sequence's end lie other sequences' rows: zeros, so that
         // nothing of them meets a product.
@@ -450,7 +475,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       arrive(&vfull[vs]);
     }
     if (!ok && lane == 0) failed();
+  }
   } else if (warp < 12) {
+    shares<ENDS, kRegS>();
     // ---- S of both heads from G, in its place: lane = token t, the blocks of 16 tokens s in turn
     if (!ENDS) {
       const int q = warp & 3, row = q * 32 + lane, odd = (warp >> 2) & 1;
@@ -518,6 +545,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!ok && lane == 0) failed();
     }
   } else if (warp < 20) {
+    shares<ENDS, kRegX>();
     // ---- the state: lane = row of the pair's 2 x 64; its columns, and blocks of 32 tokens, in two halves
     const int q = warp & 3, half = (warp >> 2) & 1 ? 0 : 1, hh = q >> 1, pr = (q & 1) * 32 + lane, prow = q * 32 + lane, head = h0 + hh;
     const bool has = head < p.heads;
@@ -666,6 +694,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     }
   } else if (!ENDS) {
+    shares<ENDS, kRegY>();
     // ---- y of one head: lane = token
     const int q = warp & 3, row = q * 32 + lane, h = (warp - 20) >> 2, head = h0 + h;
     const bool has = head < p.heads;
@@ -716,28 +745,37 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc::fence_before();
       arrive(y2scaled);
       arrive(&xempty[sl]);
+      // The gate of 16 columns is ready before their sums: the first while the
+      // products still run, the next while the next sums come from TMEM.
+      F2 gate[8];
+      const auto next_gate = [&] {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) gate[k] = silu2(f2(bf_lo(z[k]), bf_hi(z[k])));
+#pragma unroll
+        for (int i = 0; i < 24; ++i) z[i] = z[i + 8];
+      };
+      if (p.z) next_gate();
       if (!(ok = wait(yfull, c & 1) && wait(&xscan[vs], (c / kVecs) & 1))) break;
       tc::fence_after();
       const int spoilt = anybad[vs * 8 + 2 * h] | anybad[vs * 8 + 2 * h + 1] | anybad[vs * 8 + 4 + 2 * h] | anybad[vs * 8 + 4 + 2 * h + 1];
+      uint32_t r[16];
+      tc::tmem_ld16(ycol, r);
 #pragma unroll 1
       for (int j = 0; j < 4; ++j) {
-        uint32_t r[16];
-        tc::tmem_ld16(ycol + j * 16, r);
         tc::tmem_wait_ld();
         tc::landed(r);
-        if (j == 3) {
-          tc::fence_before();
-          arrive(yfree);
-        }
         uint32_t o[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          F2 y = f2(r[2 * k], r[2 * k + 1]);
-          if (p.z) y = mul2(y, silu2(f2(bf_lo(z[k]), bf_hi(z[k]))));
-          o[k] = pack_bf16(y);
+          const F2 y = f2(r[2 * k], r[2 * k + 1]);
+          o[k] = pack_bf16(p.z ? mul2(y, gate[k]) : y);
         }
-#pragma unroll
-        for (int i = 0; i < 24; ++i) z[i] = z[i + 8];  // the next columns' to the front
+        if (j < 3) {
+          tc::tmem_ld16(ycol + j * 16 + 16, r);
+        } else {
+          tc::fence_before();
+          arrive(yfree);
+        }
         if (spoilt) {
 #pragma unroll 1
           for (int i = 0; i < 16; ++i) {
@@ -752,6 +790,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                                                                 head * 64 + j * 16),
                        "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
                        : "memory");
+        if (p.z && j < 3) next_gate();
       }
       arrive(&vempty[vs]);
     }
