@@ -51,7 +51,7 @@ class TensorC(C.Structure):
 
 
 class SequencesC(C.Structure):
-    _fields_ = [("starts", C.c_void_p), ("slots", C.c_void_p), ("seqs", C.c_int32), ("tokens", C.c_int32),
+    _fields_ = [("starts", C.c_void_p), ("slots", C.c_void_p), ("order", C.c_void_p), ("seqs", C.c_int32), ("tokens", C.c_int32),
                 ("state_rows", C.c_int32), ("longest", C.c_int32)]
 
 

@@ -184,10 +184,7 @@ __global__ void __launch_bounds__(128) k_scan_seq(const ScanParams p, ScanWork w
   if (seg > 0) {
     t = seq_tile(p.plan, tile, seg);
   } else {
-    t.seq = tile;
-    t.start = t.first = p.plan.starts ? p.plan.starts[tile] : tile;
-    t.end = p.plan.starts ? p.plan.starts[tile + 1] : tile + 1;
-    t.live = t.start >= 0 && t.end <= p.plan.tokens && t.start < t.end;
+    t = seq_whole(p.plan, tile);
   }
   if (!t.live) return;
   const int slot = p.plan.slots ? p.plan.slots[t.seq] : t.seq;

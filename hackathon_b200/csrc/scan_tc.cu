@@ -167,10 +167,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (g.seg > 0) {
     t = seq_tile(p.plan, tile, g.seg);
   } else {
-    t.seq = tile;
-    t.start = t.first = p.plan.starts[tile];
-    t.end = p.plan.starts[tile + 1];
-    t.live = t.start >= 0 && t.end <= p.plan.tokens && t.start < t.end;
+    t = seq_whole(p.plan, tile);
   }
   if (!t.live) return;
   const int slot = p.plan.slots ? p.plan.slots[t.seq] : t.seq;
@@ -181,6 +178,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int end = g.seg > 0 ? min(t.end, t.first + g.seg) : t.end;
   if (ENDS && end == t.end) return;
   const int chunks = (end - t.first + Q - 1) / Q;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // What the first chunk waits for from HBM, on its way while the CTA sets up: dt,
+  // and the state's rows (half a row a thread).
+  if (warp == 2) {
+#pragma unroll
+    for (int k = 0; k < Q; k += 32)
+      if (t.first + k + lane < end)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.dt + (long long)(t.first + k + lane) * p.lddt + h0));
+  } else if (!ENDS && warp >= 12 && warp < 20) {
+    const int row = (warp & 3) * 32 + lane, half = warp >= 16;
+    if (h0 + (row >> 6) < p.heads) {
+      const bool joined = g.seg > 0 && t.end - t.start > g.seg;
+      const float* f = (joined ? g.wk.state + ((long long)tile * p.heads + h0) * 64 * N : p.ssm + ((long long)slot * p.heads + h0) * 64 * N) +
+                       (long long)row * N + half * (N / 2);
+#pragma unroll
+      for (int k = 0; k < N / 2; k += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(f + k));
+    }
+  }
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -194,7 +210,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
            *y2scaled = bar + 26, *yfull = bar + 27, *yfree = bar + 28, *hready = bar + 29, *hdone = bar + 30, *done = bar + 31;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&cbfull[i], 1);

@@ -68,6 +68,7 @@ void fp8_gemm(const Fp8GemmParams& p, cudaStream_t s);
 struct SeqPlan {
   const int* starts;
   const int* slots;
+  const int* order;  // or null: the sequences in the order that their work starts in, longest first
   int seqs, tokens, state_rows;
   int longest;  // tokens of the longest sequence
 };
@@ -155,6 +156,17 @@ __device__ __forceinline__ SeqTile seq_tile(const SeqPlan& p, int tile, int len)
   const int k = tile - (t.start / len + lo);
   t.first = t.start + k * len;
   t.live = t.start >= 0 && t.end <= p.tokens && k >= 0 && t.first < t.end;
+  return t;
+}
+
+// Tile `i` of a launch with one tile a sequence.
+__device__ __forceinline__ SeqTile seq_whole(const SeqPlan& p, int i) {
+  SeqTile t;
+  t.seq = p.order ? p.order[i] : i;
+  t.live = t.seq >= 0 && t.seq < p.seqs;
+  t.start = t.first = t.live ? p.starts[t.seq] : 0;
+  t.end = t.live ? p.starts[t.seq + 1] : 0;
+  t.live = t.live && t.start >= 0 && t.end <= p.tokens && t.start < t.end;
   return t;
 }
 

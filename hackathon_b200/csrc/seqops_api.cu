@@ -37,6 +37,7 @@ SeqPlan to_plan(const b2e_sequences* s, int rows) {
   B2E_CHECK(s->longest <= s->tokens, kErrInvalid, "the longest sequence has more tokens than the plan");
   p.starts = s->starts;
   p.slots = s->slots;
+  p.order = s->order;
   p.seqs = s->seqs;
   p.tokens = s->tokens;
   p.state_rows = s->state_rows;

@@ -193,10 +193,13 @@ class SequenceBatch:
         starts = [0]
         for n in lengths:
             starts.append(starts[-1] + n)
-        host = ([] if single else starts) + ([] if slots is None else slots)
+        order = [] if single else sorted(range(len(lengths)), key=lambda i: -lengths[i])  # longest first
+        host = ([] if single else starts) + order + ([] if slots is None else slots)
         self._arrays = torch.tensor(host, dtype=torch.int32).to(self.device)
         at = self._arrays.data_ptr()
-        self._c = _lib.SequencesC(None if single else at, None if slots is None else at + (0 if single else 4 * len(starts)),
+        order_at = at + 4 * len(starts)
+        slots_at = at if single else order_at + 4 * len(order)
+        self._c = _lib.SequencesC(None if single else at, None if slots is None else slots_at, None if single else order_at,
                                   len(lengths), self.tokens, self.state_rows, max(lengths, default=0))
 
     def __len__(self) -> int:

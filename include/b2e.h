@@ -240,6 +240,8 @@ B2E_API int b2e_linear_static(const void* x, int32_t x_dtype, int32_t m, int32_t
 typedef struct b2e_sequences {
   const int32_t* starts; /* [seqs + 1] */
   const int32_t* slots;  /* [seqs] */
+  const int32_t* order;  /* [seqs], or NULL: a permutation of the sequences that their work starts in;
+                            longest first keeps a long one from starting last */
   int32_t seqs;
   int32_t tokens;
   int32_t state_rows;

@@ -117,9 +117,9 @@ def test_sequence_batch_refuses(lengths, slots, kw, match):
 def test_sequence_batch_layout():
     b = batch([3, 0, 2], [4, 0, 1])
     assert (b.tokens, b.state_rows, len(b)) == (5, 5, 3)
-    assert b._arrays.tolist() == [0, 3, 3, 5, 4, 0, 1]
+    assert b._arrays.tolist() == [0, 3, 3, 5, 0, 2, 1, 4, 0, 1]
     assert (b._c.seqs, b._c.tokens, b._c.longest) == (3, 5, 3)
-    assert b._c.slots - b._c.starts == 16
+    assert (b._c.order - b._c.starts, b._c.slots - b._c.starts) == (16, 28)
     steps = batch([1, 1], [1, 0])  # one token a sequence: no starts
     assert steps._c.starts is None and steps._arrays.tolist() == [1, 0]
     assert batch([]).tokens == 0
@@ -154,7 +154,7 @@ def test_c_abi_refuses_before_any_device_call():
         rc, msg = call("b2e_fp8_linear", *args)
         assert rc == -1 and match in msg
     plan = lambda starts=P, slots=None, seqs=2, tokens=5, rows=2, longest=3: C.byref(  # noqa: E731
-        _lib.SequencesC(starts, slots, seqs, tokens, rows, longest))
+        _lib.SequencesC(starts, slots, None, seqs, tokens, rows, longest))
     for p, rows, taps, match in [
         (plan(tokens=6), 5, 4, "more tokens"), (plan(seqs=3), 5, 4, "more sequences"), (plan(starts=None), 5, 4, "without starts"),
         (plan(seqs=-1), 5, 4, "negative"), (plan(longest=6), 5, 4, "longest"), (plan(), 5, 5, "2 to 4 taps"),
@@ -182,7 +182,7 @@ def test_scan_workspace_follows_the_plan():
     args = _lib.ScanArgsC(rows=1 << 20, heads=8, size=64, state=128, ldx=512, ldy=512)
     def need(seqs, tokens, longest):
         out = C.c_int64(-1)
-        plan = _lib.SequencesC(1 << 20, None, seqs, tokens, seqs, longest)
+        plan = _lib.SequencesC(1 << 20, None, None, seqs, tokens, seqs, longest)
         _lib.check(_lib.lib().b2e_mamba2_scan_workspace(C.byref(plan), C.byref(args), C.byref(out)))
         return out.value
     assert need(1, 100, 100) == 0 and need(2000, 200000, 1000) == 0
