@@ -525,8 +525,10 @@ void launch_rows(const Fp8GemmParams& p, const Args& e, cudaStream_t s) {
   launch_rows_y<BN, kF16>(p, e, s);
 }
 
+// False where the scales of a CTA's groups would not fit beside the ring (k above
+// 17,000 in a projection too wide to share its groups out).
 template <int BR>
-void launch_few(const Fp8GemmParams& p, const Args& e, cudaStream_t s) {
+bool launch_few(const Fp8GemmParams& p, const Args& e, cudaStream_t s) {
   using K = FewCfg<BR>;
   CUtensorMap tx, tw;
   tc::make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.x, p.k, p.m, p.ldx, kKB, BR);
@@ -537,7 +539,7 @@ void launch_few(const Fp8GemmParams& p, const Args& e, cudaStream_t s) {
   while (split < 8 && split * 2 <= e.groups && (long long)tn * tm * split * 2 <= 148) split *= 2;
   const int per = ceil_div(e.groups, split), stages = std::min(kFewStages, per);
   const size_t smem = K::smem(stages, per);
-  B2E_CHECK(smem <= kSmemMax, kErrInvalid, "fp8_linear: k is too large");
+  if (smem > kSmemMax) return false;
   B2E_CUDA(cudaFuncSetAttribute(k_fp8_few<BR>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(tn * split, tm);
@@ -550,6 +552,7 @@ void launch_few(const Fp8GemmParams& p, const Args& e, cudaStream_t s) {
   cfg.attrs = at;
   cfg.numAttrs = 1;
   B2E_CUDA(cudaLaunchKernelEx(&cfg, k_fp8_few<BR>, tx, tw, e, stages));
+  return true;
 }
 
 }  // namespace
@@ -560,10 +563,11 @@ void fp8_gemm(const Fp8GemmParams& p, cudaStream_t s) {
   Args e{p.xs, p.ws, p.bias, p.y, p.ldy, p.m, p.n, ceil_div(p.k, kFp8Group), ceil_div(p.k, kFp8Group),
          p.relu, p.y_type, 0, 0, 0, p.err};
   e.vec = reinterpret_cast<uintptr_t>(p.y) % 32 == 0 && (p.ldy * esz) % 32 == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
-  if (p.m <= 16) return launch_few<16>(p, e, s);
-  if (p.m <= 32) return launch_few<32>(p, e, s);
-  if (p.m <= 64) return launch_few<64>(p, e, s);
+  if (p.m <= 16 && launch_few<16>(p, e, s)) return;
+  if (p.m > 16 && p.m <= 32 && launch_few<32>(p, e, s)) return;
+  if (p.m > 32 && p.m <= 64 && launch_few<64>(p, e, s)) return;
   const long tm = ceil_div(p.m, 128);
+  B2E_CHECK(tm * ceil_div(p.n, 128) <= 0x7fffffffL, kErrInvalid, "fp8_linear: too many tiles");
   // Tiles of 128 features run two CTAs an SM; tiles of 256 read less shared
   // memory a product. The wider tile where its rounds over the SMs cost less.
   const long r128 = (tm * ceil_div(p.n, 128) + 295) / 296, r256 = (tm * ceil_div(p.n, 256) + 147) / 148;

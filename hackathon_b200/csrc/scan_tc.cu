@@ -10,7 +10,8 @@
 //   Y = exp(c[t]) (C H^T) + S X
 //   H <- exp(c[T]) H + (exp(c[T] - c[s]) dt[s] X)^T B
 //
-// which is the recurrence written out over a chunk. Five products a chunk, all
+// which is the recurrence written out over a chunk (with a above zero it overflows
+// where the sum of a dt over a chunk passes 88). Five products a chunk, all
 // M = 128 in float32 TMEM accumulators: G, C H^T and the state's with N = 128
 // columns (both heads at once, so the shared-memory operands are read at the
 // rate the MMA can take), S X with its left operand in TMEM.
@@ -126,6 +127,19 @@ __device__ __forceinline__ float softplus_fast(float x) {
   r = fmaf(r, q, 2.0f);
   return fmaf(s, r, x < 0.f ? 0.f : x);
 }
+
+// The place in a ring of `size`, and its phase, after `n` uses.
+struct Turn {
+  int size, at = 0, phase = 0;
+  __device__ __forceinline__ Turn(int ring, int n = 0) : size(ring), at(n % ring), phase((n / ring) & 1) {}
+  __device__ __forceinline__ void next(int n = 1) {
+    at += n;
+    if (at >= size) {
+      at -= size;
+      phase ^= 1;
+    }
+  }
+};
 
 // Decays of one head and chunk; c in powers of two.
 struct Vec {
@@ -275,34 +289,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 0) {
     // ---- loads
     if (lane == 0) {
-      int c = 0, u = 0;
+      Turn ct(2), xt(kXSlots);
       bool ok = true;
+      int c = 0, u = 0, cbs = 0;
 #pragma unroll 1
-      for (; c < chunks && ok; ++c) {
-        const int st = c & 1, row = t.first + c * Q;
-        if (c >= 2 && !(ok = poll(&cbempty[st], ((c >> 1) & 1) ^ 1))) break;
-        uint8_t* s = smem + st * K::STAGE;
-        mbar_expect_tx(&cbfull[st], (ENDS ? 1 : 2) * K::CB);
-#pragma unroll 1
-        for (int i = 0; i < NB; ++i) {
-          tc::tma_load_2d(s + K::oB + i * kTile, &mb, i * 64, row, &cbfull[st]);
-          if (!ENDS) tc::tma_load_2d(s + K::oC + i * kTile, &mc, i * 64, row, &cbfull[st]);
-        }
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const int sl = u % kXSlots;
-          if (u >= kXSlots && !(ok = poll(&xempty[sl], ((u / kXSlots) & 1) ^ 1))) break;
-          mbar_expect_tx(&xfull[sl], kTile);
-          tc::tma_load_2d(smem + K::oX + sl * kTile, &mx, (h0 + h) * 64, row, &xfull[sl]);
+      for (int i = 0; i < 3 * chunks; ++i) {  // B and C, x of either head
+        const int row = t.first + c * Q, h = u & 1;
+        const bool cb = i - 3 * c == 0;
+        uint64_t *full = cb ? &cbfull[ct.at] : &xfull[xt.at], *empty = cb ? &cbempty[ct.at] : &xempty[xt.at];
+        if ((cb ? c >= 2 : u >= kXSlots) && !(ok = poll(empty, (cb ? ct.phase : xt.phase) ^ 1))) break;
+        mbar_expect_tx(full, cb ? (ENDS ? 1 : 2) * K::CB : kTile);
+        if (cb) {
+          uint8_t* s = smem + ct.at * K::STAGE;
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            tc::tma_load_2d(s + K::oB + n * kTile, &mb, n * 64, row, full);
+            if (!ENDS) tc::tma_load_2d(s + K::oC + n * kTile, &mc, n * 64, row, full);
+          }
+          ct.next();
+          ++cbs;
+        } else {
+          tc::tma_load_2d(smem + K::oX + xt.at * kTile, &mx, (h0 + h) * 64, row, full);
+          xt.next();
           ++u;
+          c += h;
         }
       }
-      if (!ok) {
-        failed();
-        // every load issued lands before the CTA leaves (bounded)
-        for (int i = max(0, c - 2); i < c; ++i) poll(&cbfull[i & 1], (i >> 1) & 1);
-        for (int i = max(0, u - kXSlots); i < u; ++i) poll(&xfull[i % kXSlots], (i / kXSlots) & 1);
-      }
+      if (!ok) failed();
+      // After a wait that ran out, here or in another role, the loads that were
+      // issued land before the CTA leaves (bounded); otherwise they have.
+#pragma unroll 1
+      for (int i = max(0, u - kXSlots); i < u; ++i) poll(&xfull[i % kXSlots], (i / kXSlots) & 1);
+#pragma unroll 1
+      for (int i = max(0, cbs - 2); i < cbs; ++i) poll(&cbfull[i & 1], (i >> 1) & 1);
     }
   } else if (warp == 1) {
     // ---- the state's MMAs: H += (32 tokens of the split operand)^T B
@@ -343,8 +362,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint64_t dC0 = tc::desc_k(sbase + K::oC), dB0 = tc::desc_k(sbase + K::oB), dH = tc::desc_k(sbase + K::oH),
                      dX0 = desc_mn(sbase + K::oX, kTile);
       bool ok = true;
+      Turn vt(kVecs), xscanned(kVecs), xt(kXSlots);
 #pragma unroll 1
-      for (int i = 0; i <= chunks; ++i) {
+      for (int i = 0; i <= chunks; ++i, vt.next()) {
         // Y of chunk i - 1, then G of chunk i
         const int c = i - 1, st = c & 1;
         if (i > 0) {
@@ -360,21 +380,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc::commit(y2full);
           }
           __syncwarp();
-          if (!(ok = wait(sfull, c & 1) && wait(&xscan[c % kVecs], (c / kVecs) & 1) && wait(y2scaled, c & 1))) break;
+          if (!(ok = wait(sfull, c & 1) && wait(&xscan[xscanned.at], xscanned.phase) && wait(y2scaled, c & 1))) break;
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            const int u = 2 * c + h, sl = u % kXSlots;
-            if (!(ok = wait(&xfull[sl], (u / kXSlots) & 1))) break;
+          for (int h = 0; h < 2; ++h, xt.next()) {
+            if (!(ok = wait(&xfull[xt.at], xt.phase))) break;
             tc::fence_after();
-            const uint64_t dX = tc::desc_at(dX0, sl * kTile);
+            const uint64_t dX = tc::desc_at(dX0, xt.at * kTile);
             if (tc::elect()) {
 #pragma unroll 4
               for (int k = 0; k < 8; ++k)
                 mma_ts(tmem + cY + h * 64, tmem + s_col(h, k), tc::desc_at(dX, k * 16 * 128), idesc_bf16(64, true), 1);
-              tc::commit(&xempty[sl]);
+              tc::commit(&xempty[xt.at]);
             }
             __syncwarp();
           }
+          xscanned.next();
           if (!ok) break;
           if (tc::elect()) {
             tc::commit(yfull);
@@ -383,7 +403,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           __syncwarp();
         }
         if (i < chunks) {
-          if (!(ok = wait(&vfull[i % kVecs], (i / kVecs) & 1) && wait(&cbfull[i & 1], (i >> 1) & 1))) break;
+          if (!(ok = wait(&vfull[vt.at], vt.phase) && wait(&cbfull[i & 1], (i >> 1) & 1))) break;
           tc::fence_after();
           const uint64_t a = tc::desc_at(dC0, (i & 1) * K::STAGE), b = tc::desc_at(dB0, (i & 1) * K::STAGE);
           if (tc::elect()) {
@@ -415,9 +435,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     };
     fetch(end - t.first);
     bool ok = true;
+    Turn vt(kVecs);
 #pragma unroll 1
-    for (int c = 0; c < chunks; ++c) {
-      const int st = c & 1, vs = c % kVecs, valid = min(Q, end - t.first - c * Q);
+    for (int c = 0; c < chunks; ++c, vt.next()) {
+      const int st = c & 1, vs = vt.at, valid = min(Q, end - t.first - c * Q);
       Pair cum[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -442,7 +463,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const Pair b1 = upto(3), b2 = upto(7), b3 = upto(11), total = upto(15);
       const int blk = l >> 2;
       const Pair base = blk == 0 ? Pair{0.f, 0.f} : blk == 1 ? b1 : blk == 2 ? b2 : b3;
-      if (c >= kVecs && !(ok = wait(&vempty[vs], ((c / kVecs) & 1) ^ 1))) break;
+      if (c >= kVecs && !(ok = wait(&vempty[vs], vt.phase ^ 1))) break;
       Vec& v = vec[vs * 2 + hh];
 #pragma unroll
       for (int k0 = 0; k0 < 8; k0 += 4) {
@@ -473,11 +494,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // Behind the sequence's end lie other sequences' rows: zeros, so that
         // nothing of them meets a product.
         ok = wait(&cbfull[st], (c >> 1) & 1);
+        Turn xt(kXSlots, 2 * c);
 #pragma unroll 1
-        for (int h = 0; h < 2 && ok; ++h) {
-          const int u = 2 * c + h, sl = u % kXSlots;
-          if (!(ok = wait(&xfull[sl], (u / kXSlots) & 1))) break;
-          uint4* xr = reinterpret_cast<uint4*>(smem + K::oX + sl * kTile);
+        for (int h = 0; h < 2 && ok; ++h, xt.next()) {
+          if (!(ok = wait(&xfull[xt.at], xt.phase))) break;
+          uint4* xr = reinterpret_cast<uint4*>(smem + K::oX + xt.at * kTile);
           for (int i = valid * 8 + lane; i < Q * 8; i += 32) xr[i] = make_uint4(0, 0, 0, 0);
         }
         if (!ok) break;
@@ -487,7 +508,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         fence_proxy_async();
       }
-      arrive(&vfull[vs]);
+      arrive(&vfull[vt.at]);
     }
     if (!ok && lane == 0) failed();
   }
@@ -497,10 +518,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (!ENDS) {
       const int q = warp & 3, row = q * 32 + lane, odd = (warp >> 2) & 1;
       bool ok = true;
+      Turn vt(kVecs);
 #pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
-        const int vs = c % kVecs;
-        if (!(ok = wait(&vfull[vs], (c / kVecs) & 1) && wait(gfull, c & 1))) break;
+      for (int c = 0; c < chunks; ++c, vt.next()) {
+        const int vs = vt.at;
+        if (!(ok = wait(&vfull[vs], vt.phase) && wait(gfull, c & 1))) break;
         tc::fence_after();
         const int colbase = (q == 1 ? 0 : q == 2 ? 32 : 96);
 #pragma unroll 1
@@ -570,10 +592,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const float* from = g.seg > 0 && t.end - t.start > g.seg ? part : own;
     uint8_t* hrow = smem + K::oH + prow * 128;
     bool ok = true;
+    Turn vt(kVecs), xt(kXSlots, hh);
 #pragma unroll 1
-    for (int c = 0; c < chunks; ++c) {
-      const int vs = c % kVecs, u = 2 * c + hh, sl = u % kXSlots;
-      if (!(ok = wait(&vfull[vs], (c / kVecs) & 1) && (c == 0 || (wait(hdone, (c - 1) & 1) && (ENDS || wait(y2full, (c - 1) & 1)))))) break;
+    for (int c = 0; c < chunks; ++c, vt.next(), xt.next(2)) {
+      const int vs = vt.at, sl = xt.at;
+      if (!(ok = wait(&vfull[vs], vt.phase) && (c == 0 || (wait(hdone, (c - 1) & 1) && (ENDS || wait(y2full, (c - 1) & 1)))))) break;
       tc::fence_after();
       const Vec& v = vec[vs * 2 + hh];
       const F2 total = f2(v.total, v.total);
@@ -620,7 +643,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc::fence_before();
       arrive(hready);
       // exp(c[T] - c[s]) dt[s] x[s], split over three bf16 values, tokens along the columns
-      if (!(ok = wait(&xfull[sl], (u / kXSlots) & 1))) break;
+      if (!(ok = wait(&xfull[sl], xt.phase))) break;
       const uint8_t* xs = smem + K::oX + sl * kTile + (pr & 7) * 2;
       F2 finite = f2(0.f, 0.f);
       const F2 zero = finite, minus = f2(-1.f, -1.f);
@@ -717,9 +740,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const F2 d2 = f2(d, d);
     const uint32_t ycol = tmem + lanes + cY + h * 64;
     bool ok = true;
+    Turn vt(kVecs), xt(kXSlots, h);
 #pragma unroll 1
-    for (int c = 0; c < chunks; ++c) {
-      const int vs = c % kVecs, u = 2 * c + h, sl = u % kXSlots;
+    for (int c = 0; c < chunks; ++c, vt.next(), xt.next(2)) {
+      const int vs = vt.at, sl = xt.at;
       const long long tok = t.first + c * Q + row;
       const bool in = has && t.first + c * Q + row < end;
       uint32_t z[32];
@@ -732,7 +756,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                          "=r"(z[i + 6]), "=r"(z[i + 7])
                        : "l"(zp + 2 * i));
       }
-      if (!(ok = wait(&vfull[vs], (c / kVecs) & 1) && wait(&xfull[sl], (u / kXSlots) & 1) && wait(y2full, c & 1))) break;
+      if (!(ok = wait(&vfull[vs], vt.phase) && wait(&xfull[sl], xt.phase) && wait(y2full, c & 1))) break;
       tc::fence_after();
       const Vec& v = vec[vs * 2 + h];
       const float f = ex2(v.base[q] - v.neg[row]);
@@ -760,36 +784,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc::fence_before();
       arrive(y2scaled);
       arrive(&xempty[sl]);
-      // The gate of 16 columns is ready before their sums: the first while the
-      // products still run, the next while the next sums come from TMEM.
-      F2 gate[8];
-      const auto next_gate = [&] {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) gate[k] = silu2(f2(bf_lo(z[k]), bf_hi(z[k])));
-#pragma unroll
-        for (int i = 0; i < 24; ++i) z[i] = z[i + 8];
-      };
-      if (p.z) next_gate();
-      if (!(ok = wait(yfull, c & 1) && wait(&xscan[vs], (c / kVecs) & 1))) break;
-      tc::fence_after();
-      const int spoilt = anybad[vs * 8 + 2 * h] | anybad[vs * 8 + 2 * h + 1] | anybad[vs * 8 + 4 + 2 * h] | anybad[vs * 8 + 4 + 2 * h + 1];
-      uint32_t r[16];
-      tc::tmem_ld16(ycol, r);
+      int spoilt = 0;
 #pragma unroll 1
       for (int j = 0; j < 4; ++j) {
+        // The gate of 16 columns ahead of their sums: the first while the products
+        // still run.
+        F2 gate[8];
+        if (p.z) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) gate[k] = silu2(f2(bf_lo(z[k]), bf_hi(z[k])));
+#pragma unroll
+          for (int i = 0; i < 24; ++i) z[i] = z[i + 8];
+        }
+        if (j == 0) {
+          if (!(ok = wait(yfull, c & 1) && wait(&xscan[vs], vt.phase))) break;
+          tc::fence_after();
+          spoilt = anybad[vs * 8 + 2 * h] | anybad[vs * 8 + 2 * h + 1] | anybad[vs * 8 + 4 + 2 * h] | anybad[vs * 8 + 4 + 2 * h + 1];
+        }
+        uint32_t r[16];
+        tc::tmem_ld16(ycol + j * 16, r);
         tc::tmem_wait_ld();
         tc::landed(r);
+        if (j == 3) {
+          tc::fence_before();
+          arrive(yfree);
+        }
         uint32_t o[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const F2 y = f2(r[2 * k], r[2 * k + 1]);
           o[k] = pack_bf16(p.z ? mul2(y, gate[k]) : y);
-        }
-        if (j < 3) {
-          tc::tmem_ld16(ycol + j * 16 + 16, r);
-        } else {
-          tc::fence_before();
-          arrive(yfree);
         }
         if (spoilt) {
 #pragma unroll 1
@@ -805,8 +829,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                                                                 head * 64 + j * 16),
                        "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
                        : "memory");
-        if (p.z && j < 3) next_gate();
       }
+      if (!ok) break;
       arrive(&vempty[vs]);
     }
     if (!ok && lane == 0) failed();

@@ -151,7 +151,7 @@ def linear_ref(q, scale, wq, wscale, bias, relu):
     (64, 1000, 1280, True, True, torch.float16), (65, 256, 1280, True, False, torch.float32),
     (129, 384, 77, False, True, torch.float32), (1000, 2048, 528, True, False, torch.bfloat16),
     (4096, 256, 1280, False, False, torch.float32), (300, 17000, 136, False, False, torch.float32),
-    (5, 17000, 136, False, False, torch.float32), (2500, 512, 2050, True, False, torch.float16),
+    (5, 17000, 136, False, False, torch.float32), (40, 40000, 20000, False, False, torch.bfloat16), (2500, 512, 2050, True, False, torch.float16),
 ])
 def test_fp8_linear(m, k, n, bias, relu, out):
     """A product's terms are exact in float32; a group's 128 are summed in 4 steps and the groups one
