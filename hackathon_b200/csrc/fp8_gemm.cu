@@ -512,7 +512,8 @@ void launch_rows_y(const Fp8GemmParams& p, Args e, cudaStream_t s) {
   tc::make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.k, p.n, p.ldw, kKB, BN);
   e.tiles_m = ceil_div(p.m, 128);
   e.tiles_n = ceil_div(p.n, BN);
-  B2E_CUDA(cudaFuncSetAttribute(k_fp8_rows<BN, Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(K::SMEM)));
+  static std::atomic<unsigned long long> allowed{0};
+  tc::allow_smem(k_fp8_rows<BN, Y>, K::SMEM, allowed);
   const int grid = int(std::min<long long>((long long)e.tiles_m * e.tiles_n, 148LL * K::CTAS));
   k_fp8_rows<BN, Y><<<grid, K::THREADS, K::SMEM, s>>>(tx, tw, e);
   B2E_CUDA(cudaGetLastError());
@@ -540,7 +541,8 @@ bool launch_few(const Fp8GemmParams& p, const Args& e, cudaStream_t s) {
   const int per = ceil_div(e.groups, split), stages = std::min(kFewStages, per);
   const size_t smem = K::smem(stages, per);
   if (smem > kSmemMax) return false;
-  B2E_CUDA(cudaFuncSetAttribute(k_fp8_few<BR>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  static std::atomic<unsigned long long> allowed{0};
+  tc::allow_smem(k_fp8_few<BR>, kSmemMax, allowed);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(tn * split, tm);
   cfg.blockDim = dim3(kFewThreads);

@@ -867,7 +867,8 @@ void launch(const ScanParams& p, const ScanWork& wk, int seg, cudaStream_t s) {
   TcArgs g{p, wk, seg, (p.heads + 1) / 2};
   const long long tiles = seg > 0 ? seq_tiles(p.plan, seg) : p.plan.seqs;
   B2E_CHECK(tiles * g.pairs <= 0x7fffffffLL, kErrInvalid, "mamba2_scan: too many (segment, head) pairs");
-  B2E_CUDA(cudaFuncSetAttribute(k_scan_tc<NB, ENDS>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(K::SMEM)));
+  static std::atomic<unsigned long long> allowed{0};
+  tc::allow_smem(k_scan_tc<NB, ENDS>, K::SMEM, allowed);
   k_scan_tc<NB, ENDS><<<unsigned(tiles * g.pairs), kTcThreads, K::SMEM, s>>>(mx, mb, mc, g);
   B2E_CUDA(cudaGetLastError());
 }

@@ -5,6 +5,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
+
 #include "mbarrier.cuh"
 
 namespace b2e {
@@ -107,7 +109,20 @@ __device__ __forceinline__ void landed(uint32_t (&r)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 
-// ---- host: a [rows, inner] tensor of elements of `size` bytes, row stride ld
+// ---- host
+// Lets a kernel take `bytes` of shared memory, once a device (`done`: a bit each of
+// the first 64).
+template <class F>
+inline void allow_smem(F* kernel, size_t bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  B2E_CUDA(cudaGetDevice(&dev));
+  const unsigned long long bit = 1ULL << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return;
+  B2E_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+  if (dev < 64) done.fetch_or(bit, std::memory_order_acq_rel);
+}
+
+// A [rows, inner] tensor of elements of `size` bytes, row stride ld
 // elements (a multiple of 16 bytes), read in tiles of box_inner x box_rows with
 // the 128-byte swizzle; elements outside read as zero.
 void make_map(CUtensorMap* m, CUtensorMapDataType type, int size, const void* base, uint64_t inner, uint64_t rows,

@@ -20,6 +20,7 @@ does not have: ``rms_norm_fp8``, ``fp8_linear`` with its quantisers,
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -185,6 +186,7 @@ class SequenceBatch:
         self.state_rows = need if state_rows is None else int(state_rows)
         assert need <= self.state_rows < 2 ** 31, f"slots reach row {need - 1} of {self.state_rows} state rows"
         self.lengths = tuple(lengths)
+        self.longest = max(lengths, default=0)
         self.slots = tuple(range(len(lengths))) if slots is None else tuple(slots)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
@@ -200,7 +202,7 @@ class SequenceBatch:
         order_at = at + 4 * len(starts)
         slots_at = at if single else order_at + 4 * len(order)
         self._c = _lib.SequencesC(None if single else at, None if slots is None else slots_at, None if single else order_at,
-                                  len(lengths), self.tokens, self.state_rows, max(lengths, default=0))
+                                  len(lengths), self.tokens, self.state_rows, self.longest)
 
     def __len__(self) -> int:
         return len(self.lengths)
@@ -266,9 +268,23 @@ def _vector(t, n: int, name: str, device):
     """An optional float32 vector of n values."""
     if t is None:
         return None
-    assert t.dtype == torch.float32 and tuple(t.shape) == (n,), f"{name} must be float32 ({n},), got {t.dtype} {tuple(t.shape)}"
+    assert t.dtype == torch.float32 and t.shape == (n,), f"{name} must be float32 ({n},), got {t.dtype} {tuple(t.shape)}"
     assert t.device == device, f"{name} must be on {device}, it is on {t.device}"
-    return t.contiguous()
+    return t if t.stride(0) == 1 or n == 1 else t.contiguous()
+
+
+def _operand(t: torch.Tensor, dtype, shape, name: str, device) -> None:
+    assert t.dtype == dtype and t.shape == shape, f"{name} must be {dtype} {shape}, got {t.dtype} {tuple(t.shape)}"
+    assert t.device == device, f"{name} must be on {device}, it is on {t.device}"
+
+
+def _head_rows(t: torch.Tensor):
+    """A 3-D operand (rows, heads, size) whose rows are contiguous (copied if they are not) and its row stride."""
+    n, h, p = t.shape
+    a, b, c = t.stride()
+    if (c == 1 or p == 1) and (b == p or h == 1) and (a >= h * p or n <= 1):
+        return t, (a if n > 1 else h * p)
+    return t.contiguous(), h * p
 
 
 def _on_gpu(t: torch.Tensor, name: str) -> None:
@@ -349,9 +365,8 @@ def fp8_linear(q, scale, wq, wscale, bias=None, relu: bool = False, out_dtype=to
     m, k = q.shape
     n, g = wq.shape[0], -(-k // FP8_GROUP)
     dev = q.device
-    for t, shape, name in ((scale, (m, g), "scale"), (wscale, (-(-n // FP8_GROUP), g), "wscale")):
-        assert t.dtype == torch.float32 and tuple(t.shape) == shape, f"{name} must be float32 {shape}, got {t.dtype} {tuple(t.shape)}"
-        assert t.device == dev, f"{name} must be on {dev}, it is on {t.device}"
+    _operand(scale, torch.float32, (m, g), "scale", dev)
+    _operand(wscale, torch.float32, (-(-n // FP8_GROUP), g), "wscale", dev)
     assert wq.device == dev, f"wq must be on {dev}, it is on {wq.device}"
     assert out_dtype in _TORCH_DTYPES, f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}"
     bias = _vector(bias, n, "bias", dev)
@@ -402,9 +417,7 @@ def causal_conv(window, x, weight, bias=None, seqs: Optional[SequenceBatch] = No
     assert ch > 0 and x.dim() == 2 and x.shape[1] == ch, f"x must be (rows, {ch}), got {tuple(x.shape)}"
     xt = _float(x, "x")
     assert x.device == dev, f"x must be on {dev}, it is on {x.device}"
-    assert weight.dtype == torch.float32 and tuple(weight.shape) == (ch, taps), \
-        f"weight must be float32 {(ch, taps)}, got {weight.dtype} {tuple(weight.shape)}"
-    assert weight.device == dev, f"weight must be on {dev}, it is on {weight.device}"
+    _operand(weight, torch.float32, (ch, taps), "weight", dev)
     bias = _vector(bias, ch, "bias", dev)
     rows = x.shape[0]
     plan, tokens = _plan(seqs, rows, window, "window")
@@ -416,6 +429,10 @@ def causal_conv(window, x, weight, bias=None, seqs: Optional[SequenceBatch] = No
         _call("b2e_causal_conv", dev, plan, _at(window), _at(x), xt, ldx, rows, ch, _at(weight), _at(bias), taps, int(silu),
               _at(y), ch)
     return y
+
+
+_SCAN_ARGS = struct.Struct("9Q6q6i")
+assert _SCAN_ARGS.size == C.sizeof(_lib.ScanArgsC)
 
 
 def mamba2_scan(ssm, x, b, c, dt, a, seqs: Optional[SequenceBatch] = None, d=None, z=None, softplus: bool = True):
@@ -432,33 +449,35 @@ def mamba2_scan(ssm, x, b, c, dt, a, seqs: Optional[SequenceBatch] = None, d=Non
     _scan_state_ok(ssm)
     nrows, h, p, n = ssm.shape
     dev = ssm.device
-    assert x.dim() == 3 and tuple(x.shape[1:]) == (h, p), f"x must be (rows, {h}, {p}), got {tuple(x.shape)}"
+    assert x.dim() == 3, f"x must be (rows, {h}, {p}), got {tuple(x.shape)}"
+    rows, dtype = x.shape[0], x.dtype
     xt = _float(x, "x")
-    rows = x.shape[0]
-    for t, shape, name in ((x, (rows, h, p), "x"), (z, (rows, h, p), "z"), (b, (rows, n), "b"), (c, (rows, n), "c")):
-        if t is not None:
-            assert t.dtype == x.dtype and tuple(t.shape) == shape, f"{name} must be {x.dtype} {shape}, got {t.dtype} {tuple(t.shape)}"
-            assert t.device == dev, f"{name} must be on {dev}, it is on {t.device}"
-    assert dt.dtype == torch.float32 and tuple(dt.shape) == (rows, h), f"dt must be float32 {(rows, h)}, got {dt.dtype} {tuple(dt.shape)}"
-    assert dt.device == dev, f"dt must be on {dev}, it is on {dt.device}"
+    _operand(x, dtype, (rows, h, p), "x", dev)
+    if z is not None:
+        _operand(z, dtype, (rows, h, p), "z", dev)
+    _operand(b, dtype, (rows, n), "b", dev)
+    _operand(c, dtype, (rows, n), "c", dev)
+    _operand(dt, torch.float32, (rows, h), "dt", dev)
     assert a is not None, "a must be given"
     a, d = _vector(a, h, "a", dev), _vector(d, h, "d", dev)
     plan, tokens = _plan(seqs, rows, ssm, "ssm")
     _on_gpu(ssm, "ssm")
     y = _out(x, rows, tokens)
     if tokens:
-        x, ldx = _rows(x.reshape(rows, h * p))
-        z, ldz = (None, 0) if z is None else _rows(z.reshape(rows, h * p))
+        x, ldx = _head_rows(x)
+        z, ldz = (None, 0) if z is None else _head_rows(z)
         (b, ldb), (c, ldc), (dt, lddt) = _rows(b), _rows(c), _rows(dt)
-        args = _lib.ScanArgsC(ssm.data_ptr(), x.data_ptr(), b.data_ptr(), c.data_ptr(), dt.data_ptr(), a.data_ptr(), _at(d),
-                              _at(z), y.data_ptr(), ldx, ldb, ldc, lddt, ldz, h * p, rows, h, p, n, xt, int(softplus))
-        ref, work, size = C.byref(args), None, 0
-        if seqs is not None:
+        # b2e_scan_args, packed (a ctypes structure takes as long as the launch)
+        args = _SCAN_ARGS.pack(ssm.data_ptr(), x.data_ptr(), b.data_ptr(), c.data_ptr(), dt.data_ptr(), a.data_ptr(),
+                               0 if d is None else d.data_ptr(), 0 if z is None else z.data_ptr(), y.data_ptr(),
+                               ldx, ldb, ldc, lddt, ldz, h * p, rows, h, p, n, xt, softplus)
+        work, size = None, 0
+        if seqs is not None and seqs.longest > 1:
             need = C.c_int64()
-            _lib.check(_lib.lib().b2e_mamba2_scan_workspace(plan, ref, C.byref(need)))
+            _lib.check(_lib.lib().b2e_mamba2_scan_workspace(plan, args, C.byref(need)))
             size = need.value
             work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        _call("b2e_mamba2_scan", dev, plan, ref, _at(work), size)
+        _call("b2e_mamba2_scan", dev, plan, args, _at(work), size)
     return y
 
 
