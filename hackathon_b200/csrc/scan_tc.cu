@@ -591,6 +591,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     float* part = g.wk.state + ((long long)tile * p.heads + head) * hp + (long long)pr * N;
     const float* from = g.seg > 0 && t.end - t.start > g.seg ? part : own;
     uint8_t* hrow = smem + K::oH + prow * 128;
+    // the state that the segment starts from, while the first chunk's decays are made
+#pragma unroll 1
+    for (int j = half * (N / 32); j < (half + 1) * (N / 32); ++j) {
+      uint32_t r[16];
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const float4 f = !ENDS && has ? *reinterpret_cast<const float4*>(from + j * 16 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        r[i] = __float_as_uint(f.x);
+        r[i + 1] = __float_as_uint(f.y);
+        r[i + 2] = __float_as_uint(f.z);
+        r[i + 3] = __float_as_uint(f.w);
+      }
+      tc::tmem_st16(tmem + lanes + cH + j * 16, r);
+    }
+    tc::tmem_wait_st();
     bool ok = true;
     Turn vt(kVecs), xt(kXSlots, hh);
 #pragma unroll 1
@@ -603,20 +618,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 1
       for (int j = half * (N / 32); j < (half + 1) * (N / 32); ++j) {
         uint32_t r[16];
-        if (c > 0) {
-          tc::tmem_ld16(tmem + lanes + cH + j * 16, r);
-          tc::tmem_wait_ld();
-          tc::landed(r);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const float4 f = !ENDS && has ? *reinterpret_cast<const float4*>(from + j * 16 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-            r[i] = __float_as_uint(f.x);
-            r[i + 1] = __float_as_uint(f.y);
-            r[i + 2] = __float_as_uint(f.z);
-            r[i + 3] = __float_as_uint(f.w);
-          }
-        }
+        tc::tmem_ld16(tmem + lanes + cH + j * 16, r);
+        tc::tmem_wait_ld();
+        tc::landed(r);
         if (!ENDS) {
 #pragma unroll
           for (int i = 0; i < 16; i += 8) {
