@@ -38,10 +38,10 @@ template <int T>
 __device__ __forceinline__ void load8(const void* p, long long i, float (&v)[8]) {
   if constexpr (T == kF32) {
     const float4* f = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
-    const float4 a = __ldcs(f), b = __ldcs(f + 1);
+    const float4 a = __ldg(f), b = __ldg(f + 1);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
-    const uint4 r = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i));
+    const uint4 r = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i));
     const uint32_t u[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(256) k_rms_fp8(const RmsFp8Params p) {
       uint2 o;
       o.x = to_e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
       o.y = to_e4m3x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
-      *reinterpret_cast<uint2*>(p.q + row * p.ldq + u * 8) = o;
+      __stcs(reinterpret_cast<uint2*>(p.q + row * p.ldq + u * 8), o);
       if (u % 16 == 0) p.scale[(long long)row * groups + u / 16] = scale;
     }
   }
