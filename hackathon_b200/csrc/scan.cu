@@ -154,15 +154,28 @@ __global__ void __launch_bounds__(256) k_scan_step_any(const ScanParams p) {
 //
 // A CTA of 128 threads walks one segment of a sequence for one head and 8 R state
 // rows. Sixteen lanes cover a row, a thread holds R rows by J vectors of four
-// columns (interleaved by lane) in registers. Bound by the FP32 pipe: three
-// operations a state element and token, two elements an instruction. The layout
-// keeps shared memory off that path: a token costs a thread 2 J + R / 4 vectors
-// (with two rows and 32 columns a thread it was 16, and LDS was the limit: 294 us
-// for 64 sequences of 10000 tokens, 8 heads, against 218 us). Tokens are staged in
-// blocks of 16, the next block by cp.async while one is computed where the
-// operands are float32 vectors.
+// columns (interleaved by lane) in registers. The decay of a token is one scalar
+// for the whole head, so the registers hold H = h / P with P the product of the
+// decays since it was last 1:
+//
+//   P <- decay P;  H <- H + (dt / P) x b^T;  y = P (H c)
+//
+// two operations a state element and token instead of three, and one instead of
+// two where only the state is wanted. P is multiplied into H when it leaves
+// [2^-12, 2^12] (P and the token's decay one after the other, as h would have
+// been multiplied) and at the end, so dt x b has 2^12 of headroom less than
+// float32's range, and a decay is rounded into P as it would be into h.
+//
+// Bound by the FP32 pipe (two elements an instruction, two cycles each) and, a
+// third of the issue slots, the exchange of row sums. The layout keeps shared
+// memory off that path: a token costs a thread 2 J + R / 4 vectors. 64 sequences of
+// 10000 tokens in all, 8 heads of 64 x 128, float32: 195 us; 220 with three
+// operations, 204 with four rows a thread, 294 with two rows and 32 columns, where
+// shared memory bound it. Tokens are staged in blocks of 16, the next block by
+// cp.async while one is computed where the operands are float32 vectors.
 
 constexpr int kTok = 16;  // tokens staged together
+constexpr float kLowP = 0x1p-12f;  // bounds of P
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {  // zeros behind `bytes`
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(uint32_t(__cvta_generic_to_shared(dst))), "l"(src), "r"(bytes)
@@ -268,6 +281,17 @@ __global__ void __launch_bounds__(128) k_scan_seq(const ScanParams p, ScanWork w
       H[i][j][1] = f2(v.z, v.w);
     }
   float logsum = 0.f;  // of thread 0: log of the segment's decay
+  float P = 1.f;       // the state is P H
+  const auto scale_state = [&](float f) {
+    const F2 f2x = f2(f, f);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        H[i][j][0] = mul2(H[i][j][0], f2x);
+        H[i][j][1] = mul2(H[i][j][1], f2x);
+      }
+  };
   int buf = 0;
   for (int t0 = t.first; t0 < end; t0 += kTok) {
     const int n = min(kTok, end - t0);
@@ -289,8 +313,14 @@ __global__ void __launch_bounds__(128) k_scan_seq(const ScanParams p, ScanWork w
       for (int k = 0; k < n; ++k) logsum += av * sdt[buf][k];
 #pragma unroll 1
     for (int k = 0; k < n; ++k) {
-      const float dt = sdt[buf][k], dc = sdec[buf][k];
-      const F2 dc2 = f2(dc, dc);
+      const float dc = sdec[buf][k], pn = P * dc;
+      const bool keep = pn >= kLowP && pn <= 1.f / kLowP;  // not for a NaN
+      if (!keep) {
+        scale_state(P);
+        scale_state(dc);
+      }
+      P = keep ? pn : 1.f;
+      const float dt = sdt[buf][k] * rcp(P);
       F2 u[R], y[R];
 #pragma unroll
       for (int i = 0; i < R; i += 4) {
@@ -309,8 +339,8 @@ __global__ void __launch_bounds__(128) k_scan_seq(const ScanParams p, ScanWork w
         const F2 b0 = f2(b4.x, b4.y), b1 = f2(b4.z, b4.w), c0 = f2(c4.x, c4.y), c1 = f2(c4.z, c4.w);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-          H[i][j][0] = fma2(dc2, H[i][j][0], mul2(u[i], b0));
-          H[i][j][1] = fma2(dc2, H[i][j][1], mul2(u[i], b1));
+          H[i][j][0] = fma2(u[i], b0, H[i][j][0]);
+          H[i][j][1] = fma2(u[i], b1, H[i][j][1]);
           if (!ends) {
             y[i] = fma2(c0, H[i][j][0], y[i]);
             y[i] = fma2(c1, H[i][j][1], y[i]);
@@ -327,7 +357,7 @@ __global__ void __launch_bounds__(128) k_scan_seq(const ScanParams p, ScanWork w
         }
         int which;
         const float v = group_sums<16, R>(sums, lane, which);
-        if (c16 % (16 / R) == 0) sy[k][rg * R + which] = v;
+        if (c16 % (16 / R) == 0) sy[k][rg * R + which] = P * v;
       }
     }
     if (ASYNC && t0 + kTok < end) decays(next, buf ^ 1);
@@ -346,6 +376,7 @@ __global__ void __launch_bounds__(128) k_scan_seq(const ScanParams p, ScanWork w
   }
   if (ends && threadIdx.x == 0 && p0 == 0) wk.log_decay[(long long)tile * p.heads + h] = logsum;
   if (ends || end == t.end) {
+    scale_state(P);
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
@@ -515,7 +546,8 @@ ScanWork scan_work(const ScanParams& p, int seg) {
 // an SM, one of the chunked kernel). Segments then are that even share in blocks
 // of 128 tokens: rounded down for the recurrence kernel, whose CTAs queue, up for
 // the chunked one, where one CTA too many is a second wave. 64 sequences of 10000
-// tokens in all (up to 700), 8 heads, float32: 314 us whole, 218 us split.
+// tokens in all (up to 700), 8 heads, float32: 288 us whole, 195 us split in 128
+// tokens, 254 us in 256.
 int scan_segment(const ScanParams& p) {
   if (single_tokens(p)) return 0;
   const bool tc = scan_tc_eligible(p);

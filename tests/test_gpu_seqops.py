@@ -369,6 +369,19 @@ def test_mamba2_scan_decays(dt, kind):
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=ids)
+@pytest.mark.parametrize("n", [40, 100, 200])
+def test_mamba2_scan_products_of_decays(dt, n):
+    """Products of a sequence's decays far above and far below one, in small steps and in large ones."""
+    inp = scan_inputs(12, 3, 160, 2, 48, n, dt, False)
+    steps = torch.full((160, 2), 0.6, device=DEV)
+    steps[:40] = -0.6                # up by e^24 and down again, then as far below
+    steps[80:100] = 9.0              # each decay below the range that is kept on
+    steps[100:120] = -1.0
+    inp["dt"], inp["a"] = steps, torch.tensor([-1.0, -0.3], device=DEV)
+    check_scan(inp, [100, 20, 40], None, 3, 160, pairs=0.0, softplus=False)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=ids)
 @pytest.mark.parametrize("name", ["x", "b", "c", "dt"])
 def test_mamba2_scan_values_that_are_not_finite_stay_behind(dt, name):
     """A NaN or an infinity in a token reaches neither earlier tokens nor other sequences or heads' rows."""
