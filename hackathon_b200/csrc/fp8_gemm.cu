@@ -13,14 +13,21 @@
 // Two shapes of the same pipeline:
 //  - rows kernel: M = 128 activation rows (a thread's TMEM lane is a row, so both
 //    scales are one scalar a thread and group), N = BN output features;
-//    persistent CTAs. Bound by the tensor cores: a group costs 128 x BN x 128
-//    products, its epilogue BN / 2 FMAs a thread of eight warps.
+//    persistent CTAs. Bound by the exchange of the accumulators: a group of BN =
+//    256 takes the tensor cores 515 cycles, and its sums, read from TMEM and
+//    scaled by eight warps (128 FMAs a thread), about 800. 18944 x 4096 x 4096 to
+//    bf16 takes 322 us (1.97 PFLOP/s), 10000 x 4096 x 2048 101 us (1.66), where a
+//    last round of whole tiles over the SMs would leave most of them idle: tiles
+//    that would are taken in halves (104 us without; 4096 x 256 x 1280 13.5 us
+//    for 14.8, 300 x 2048 x 8448 18.0 for 19.4).
 //  - few-rows kernel: M = 128 output features, N = BR <= 64 rows; the groups are
 //    shared out over a cluster of up to 8 CTAs, whose float32 sums meet through
 //    distributed shared memory in rank order (the same result every time). Bound
-//    by the weight's bytes.
+//    by latency at the sizes it is for: 1 x 2048 x 8448 takes 7.9 us, 2.7 of them
+//    its weight's bytes, the rest the first load, the joining and the launch.
 #include <algorithm>
 #include <cooperative_groups.h>
+#include <type_traits>
 
 #include "seqops.cuh"
 #include "tc.cuh"
@@ -56,6 +63,7 @@ struct Args {
   int m, n, groups, wgroups;  // wgroups: scale columns of ws
   int relu, y_type, vec;      // vec: rows of y may take 32-byte stores
   int tiles_m, tiles_n;
+  int whole;  // rows kernel: tiles behind the first `whole` are taken in two halves
   int* err;
 };
 
@@ -119,6 +127,18 @@ struct RowsCfg {
   static constexpr size_t SMEM = size_t(STAGES) * STAGE + SCALES + 1024 + 256;
 };
 
+// Item `i` of the rows kernel: a tile, or half of one (its first or second 128 features).
+struct RowsItem {
+  int m0, n0;
+  bool half;
+};
+template <int BN>
+__device__ __forceinline__ RowsItem rows_item(const Args& e, int i) {
+  const bool half = BN == 256 && i >= e.whole;
+  const int t = half ? e.whole + (i - e.whole) / 2 : i;
+  return {(t % e.tiles_m) * 128, (t / e.tiles_m) * BN + (half ? (i - e.whole) % 2 * 128 : 0), half};
+}
+
 template <int BN, int Y>
 __global__ void __launch_bounds__(RowsCfg<BN>::THREADS, RowsCfg<BN>::CTAS)
     k_fp8_rows(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, const Args e) {
@@ -156,15 +176,15 @@ __global__ void __launch_bounds__(RowsCfg<BN>::THREADS, RowsCfg<BN>::CTAS)
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int tiles = e.tiles_m * e.tiles_n;
+  const int items = BN == 256 ? 2 * e.tiles_m * e.tiles_n - e.whole : e.tiles_m * e.tiles_n;
 
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(K::LOW));
   if (warp == 0) {
     if (lane == 0) {
       int it = 0;
-      for (int t = blockIdx.x; t < tiles && !*abort_flag; t += gridDim.x) {
-        const int m0 = (t % e.tiles_m) * 128, n0 = (t / e.tiles_m) * BN;
+      for (int t = blockIdx.x; t < items && !*abort_flag; t += gridDim.x) {
+        const RowsItem w = rows_item<BN>(e, t);
         for (int g = 0; g < e.groups; ++g, ++it) {
           const int s = it % S;
           if (it >= S && !mbar_wait(&empty[s], ((it / S) & 1) ^ 1, abort_flag)) {
@@ -173,9 +193,10 @@ __global__ void __launch_bounds__(RowsCfg<BN>::THREADS, RowsCfg<BN>::CTAS)
             break;
           }
           uint8_t* st = smem + size_t(s) * K::STAGE;
-          mbar_expect_tx(&full[s], K::STAGE);
-          tc::tma_load_2d(st, &tx, g * int(kKB), m0, &full[s]);
-          tc::tma_load_2d(st + K::TILE_X, &tw, g * int(kKB), n0, &full[s]);
+          mbar_expect_tx(&full[s], w.half ? K::TILE_X + K::TILE_W / 2 : K::STAGE);
+          tc::tma_load_2d(st, &tx, g * int(kKB), w.m0, &full[s]);
+          tc::tma_load_2d(st + K::TILE_X, &tw, g * int(kKB), w.n0, &full[s]);
+          if (BN == 256 && !w.half) tc::tma_load_2d(st + K::TILE_X + 128 * kKB, &tw, g * int(kKB), w.n0 + 128, &full[s]);
         }
       }
       if (*abort_flag) {  // every load issued lands before the CTA leaves (bounded)
@@ -184,11 +205,11 @@ __global__ void __launch_bounds__(RowsCfg<BN>::THREADS, RowsCfg<BN>::CTAS)
       }
     }
   } else if (warp == 1) {
-    const uint32_t idesc = idesc_f8(BN);
     const uint64_t dx0 = tc::desc_k(smem_u32(smem)), dw0 = tc::desc_k(smem_u32(smem) + K::TILE_X);
     int it = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    for (int t = blockIdx.x; t < items && ok; t += gridDim.x) {
+      const uint32_t idesc = BN == 256 && t >= e.whole ? idesc_f8(BN / 2) : idesc_f8(BN);
 #pragma unroll 1
       for (int g = 0; g < e.groups; ++g, ++it) {
         const int s = it % S, b = it & 1;
@@ -222,19 +243,20 @@ __global__ void __launch_bounds__(RowsCfg<BN>::THREADS, RowsCfg<BN>::CTAS)
     const int ew = warp - 4, fg = lane % kXB, fr = ew * 16 + lane / kXB;
     float fetched[8];
     const auto fetch = [&](int t, int g0) {
-      const int m0 = (t % e.tiles_m) * 128;
+      const int m0 = rows_item<BN>(e, t).m0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = m0 + fr + 2 * i;
         fetched[i] = r < e.m && g0 + fg < e.groups ? e.xs[(long long)r * e.groups + g0 + fg] : 0.f;
       }
     };
-    if (int(blockIdx.x) < tiles) fetch(blockIdx.x, 0);
+    if (int(blockIdx.x) < items) fetch(blockIdx.x, 0);
     int it = 0;
     bool ok = true;  // false: this warp computes and stores nothing more, but keeps to the barriers
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-      const int m0 = (t % e.tiles_m) * 128, n0 = (t / e.tiles_m) * BN;
-      const int row = m0 + q * 32 + lane, c0 = n0 + part * HN;
+    const auto item = [&](int t, auto columns) {  // of this warp
+      constexpr int HN = decltype(columns)::value;
+      const RowsItem w = rows_item<BN>(e, t);
+      const int row = w.m0 + q * 32 + lane, c0 = w.n0 + part * HN;
       const bool in = row < e.m;
       const float* ws = e.ws + (long long)(min(c0, e.n - 1) / kFp8Group) * e.wgroups;
       float2 acc[HN / 2];
@@ -251,7 +273,7 @@ __global__ void __launch_bounds__(RowsCfg<BN>::THREADS, RowsCfg<BN>::CTAS)
           named_bar(1, 32 * K::EPI);
           if (g + kXB < e.groups)
             fetch(t, g + kXB);
-          else if (t + int(gridDim.x) < tiles)
+          else if (t + int(gridDim.x) < items)
             fetch(t + gridDim.x, 0);
         }
         const float f = xsm[(g % kXB) * kXStride + q * 32 + lane] * wn;
@@ -322,6 +344,12 @@ __global__ void __launch_bounds__(RowsCfg<BN>::THREADS, RowsCfg<BN>::CTAS)
           }
         }
       }
+    };
+    for (int t = blockIdx.x; t < items; t += gridDim.x) {
+      if (BN == 256 && t >= e.whole)
+        item(t, std::integral_constant<int, HN / 2>{});
+      else
+        item(t, std::integral_constant<int, HN>{});
     }
   }
   tc::fence_before();
@@ -504,17 +532,26 @@ __global__ void __launch_bounds__(kFewThreads)
 
 constexpr size_t kSmemMax = 227 * 1024;
 
+// Tiles of 256 features left for a last round over the SMs that may as well be
+// taken in halves, because twice as many items still fit in it.
+int halved(long long tiles) {
+  const int left = int(tiles % 148);
+  return left * 2 <= 148 ? left : 0;
+}
+
 template <int BN, int Y>
 void launch_rows_y(const Fp8GemmParams& p, Args e, cudaStream_t s) {
   using K = RowsCfg<BN>;
   CUtensorMap tx, tw;
   tc::make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.x, p.k, p.m, p.ldx, kKB, 128);
-  tc::make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.k, p.n, p.ldw, kKB, BN);
+  tc::make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.k, p.n, p.ldw, kKB, 128);
   e.tiles_m = ceil_div(p.m, 128);
   e.tiles_n = ceil_div(p.n, BN);
   static std::atomic<unsigned long long> allowed{0};
   tc::allow_smem(k_fp8_rows<BN, Y>, K::SMEM, allowed);
-  const int grid = int(std::min<long long>((long long)e.tiles_m * e.tiles_n, 148LL * K::CTAS));
+  const int tiles = e.tiles_m * e.tiles_n;
+  e.whole = BN == 256 ? tiles - halved(tiles) : tiles;
+  const int grid = int(std::min<long long>(2LL * tiles - e.whole, 148LL * K::CTAS));
   k_fp8_rows<BN, Y><<<grid, K::THREADS, K::SMEM, s>>>(tx, tw, e);
   B2E_CUDA(cudaGetLastError());
 }
@@ -563,17 +600,18 @@ void fp8_gemm(const Fp8GemmParams& p, cudaStream_t s) {
   if (p.m == 0) return;
   const int esz = int(dtype_size(p.y_type));
   Args e{p.xs, p.ws, p.bias, p.y, p.ldy, p.m, p.n, ceil_div(p.k, kFp8Group), ceil_div(p.k, kFp8Group),
-         p.relu, p.y_type, 0, 0, 0, p.err};
+         p.relu, p.y_type, 0, 0, 0, 0, p.err};
   e.vec = reinterpret_cast<uintptr_t>(p.y) % 32 == 0 && (p.ldy * esz) % 32 == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
   if (p.m <= 16 && launch_few<16>(p, e, s)) return;
   if (p.m > 16 && p.m <= 32 && launch_few<32>(p, e, s)) return;
   if (p.m > 32 && p.m <= 64 && launch_few<64>(p, e, s)) return;
-  const long tm = ceil_div(p.m, 128);
-  B2E_CHECK(tm * ceil_div(p.n, 128) <= 0x7fffffffL, kErrInvalid, "fp8_linear: too many tiles");
-  // Tiles of 128 features run two CTAs an SM; tiles of 256 read less shared
-  // memory a product. The wider tile where its rounds over the SMs cost less.
-  const long r128 = (tm * ceil_div(p.n, 128) + 295) / 296, r256 = (tm * ceil_div(p.n, 256) + 147) / 148;
-  if (r256 <= r128)
+  const long long tm = ceil_div(p.m, 128), t128 = tm * ceil_div(p.n, 128), t256 = tm * ceil_div(p.n, 256);
+  B2E_CHECK(t128 <= 0x3fffffffLL, kErrInvalid, "fp8_linear: too many tiles");
+  // Tiles of 128 features run two CTAs an SM; tiles of 256 read less shared memory
+  // a product. The wider tile where its rounds over the SMs, a last one of halves
+  // counted half, cost no more.
+  const long long h128 = (t128 + 295) / 296 * 2, h256 = (t256 + 147) / 148 * 2 - (halved(t256) > 0);
+  if (h256 <= h128)
     launch_rows<256>(p, e, s);
   else
     launch_rows<128>(p, e, s);
