@@ -20,10 +20,11 @@
 //    last round of whole tiles over the SMs would leave most of them idle: tiles
 //    that would are taken in halves (104 us without; 4096 x 256 x 1280 13.5 us
 //    for 14.8, 300 x 2048 x 8448 18.0 for 19.4).
-//  - few-rows kernel: M = 128 output features, N = BR <= 64 rows; the groups are
+//  - few-rows kernel, where there are not tiles for every SM: M = 128 output
+//    features, N = BR rows (16, 32 or 64; a grid of them above 64); the groups are
 //    shared out over a cluster of up to 8 CTAs, whose float32 sums meet through
 //    distributed shared memory in rank order (the same result every time). Bound
-//    by latency at the sizes it is for: 1 x 2048 x 8448 takes 7.9 us, 2.7 of them
+//    by latency at the sizes it is for: 1 x 2048 x 8448 takes 7.6 us, 2.7 of them
 //    its weight's bytes, the rest the first load, the joining and the launch.
 #include <algorithm>
 #include <cooperative_groups.h>
@@ -359,8 +360,8 @@ __global__ void __launch_bounds__(RowsCfg<BN>::THREADS, RowsCfg<BN>::CTAS)
 
 // --------------------------------------------------------- few-rows kernel
 
-constexpr int kFewStages = 8;
-constexpr int kFewThreads = 64 + 128;
+constexpr int kFewStages = 4;  // 8, one CTA an SM, left clusters to a second round: 1 x 16384 x 2048 21.5 us against 12.4
+constexpr int kFewThreads = 64 + 128, kFewSplit = 8;  // CTAs of a cluster at most
 
 template <int BR>
 struct FewCfg {
@@ -516,16 +517,32 @@ __global__ void __launch_bounds__(kFewThreads)
     for (int j = 0; j < BR; ++j) part[j * 128 + f] = acc[j];
   }
   cl.sync();
-  // rank r sums the rows r, r + nsplit, ... over the ranks in order
+  // Rank r sums the rows r, r + nsplit, ... over the ranks in order, a warp a row,
+  // with the sums of all ranks in flight together (one read after the other, 64
+  // rows took 9 us more than one).
   const int rows = min(BR, e.m - m0);
-  for (int i = threadIdx.x; i < BR * 128; i += kFewThreads) {
-    const int r = i / 128, f = i % 128, n = n0 + f;
-    if (r >= rows || r % nsplit != rank || n >= e.n) continue;
-    float v = 0.f;
-    for (int k = 0; k < nsplit; ++k) v += cl.map_shared_rank(part, k)[i];
-    if (e.bias) v += e.bias[n];
-    if (e.relu) v = v < 0.f ? 0.f : v;
-    store_as(e.y_type, e.y, size_t((long long)(m0 + r) * e.ldy + n), v);
+#pragma unroll 1
+  for (int r = rank + nsplit * warp; r < rows; r += nsplit * (kFewThreads / 32)) {
+    float v[kFewSplit][4];
+#pragma unroll
+    for (int k = 0; k < kFewSplit; ++k)
+      if (k < nsplit) {
+        const float* from = cl.map_shared_rank(part, k) + r * 128 + lane;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[k][j] = from[32 * j];
+      }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + 32 * j + lane;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kFewSplit; ++k)
+        if (k < nsplit) sum += v[k][j];
+      if (n >= e.n) continue;
+      if (e.bias) sum += e.bias[n];
+      if (e.relu) sum = sum < 0.f ? 0.f : sum;
+      store_as(e.y_type, e.y, size_t((long long)(m0 + r) * e.ldy + n), sum);
+    }
   }
   cl.sync();  // peers' sums stay until everyone has read them
 }
@@ -563,21 +580,27 @@ void launch_rows(const Fp8GemmParams& p, const Args& e, cudaStream_t s) {
   launch_rows_y<BN, kF16>(p, e, s);
 }
 
-// False where the scales of a CTA's groups would not fit beside the ring (k above
-// 17,000 in a projection too wide to share its groups out).
+// False where the rows kernel takes less time. With one round of tiles over the SMs
+// that kernel takes 3 + 0.385 us a group, and this one 4 (one row) to 5.4 (64 rows)
+// + 0.5 us a group of its share, which is the comparison below. Rows against few:
+// 1 x 256 x 1280 3.8 / 4.2 us, 1 x 2048 x 8448 9.4 / 7.6, 64 x 2048 x 8448 9.7 /
+// 10.6, 64 x 4096 x 1024 15.5 / 7.3, 400 x 4096 x 1024 16.1 / 14.8, 1000 x 4096 x
+// 1024 16.7 / 25.4, 1 x 4096 x 40000 (more than L2) 42.4 / 43.4.
+// False too where the scales of a CTA's groups would not fit beside the ring.
 template <int BR>
 bool launch_few(const Fp8GemmParams& p, const Args& e, cudaStream_t s) {
   using K = FewCfg<BR>;
-  CUtensorMap tx, tw;
-  tc::make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.x, p.k, p.m, p.ldx, kKB, BR);
-  tc::make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.k, p.n, p.ldw, kKB, 128);
   const int tn = ceil_div(p.n, 128), tm = ceil_div(p.m, BR);
   // as many CTAs of a cluster as fill the SMs and still have a group each
   int split = 1;
-  while (split < 8 && split * 2 <= e.groups && (long long)tn * tm * split * 2 <= 148) split *= 2;
+  while (split < kFewSplit && split * 2 <= e.groups && (long long)tn * tm * split * 2 <= 148) split *= 2;
   const int per = ceil_div(e.groups, split), stages = std::min(kFewStages, per);
+  if (3LL * e.groups - 4LL * per < 8 + std::min(p.m, 64) / 7) return false;
   const size_t smem = K::smem(stages, per);
   if (smem > kSmemMax) return false;
+  CUtensorMap tx, tw;
+  tc::make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.x, p.k, p.m, p.ldx, kKB, BR);
+  tc::make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.k, p.n, p.ldw, kKB, 128);
   static std::atomic<unsigned long long> allowed{0};
   tc::allow_smem(k_fp8_few<BR>, kSmemMax, allowed);
   cudaLaunchConfig_t cfg{};
@@ -604,7 +627,7 @@ void fp8_gemm(const Fp8GemmParams& p, cudaStream_t s) {
   e.vec = reinterpret_cast<uintptr_t>(p.y) % 32 == 0 && (p.ldy * esz) % 32 == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
   if (p.m <= 16 && launch_few<16>(p, e, s)) return;
   if (p.m > 16 && p.m <= 32 && launch_few<32>(p, e, s)) return;
-  if (p.m > 32 && p.m <= 64 && launch_few<64>(p, e, s)) return;
+  if (p.m > 32 && launch_few<64>(p, e, s)) return;
   const long long tm = ceil_div(p.m, 128), t128 = tm * ceil_div(p.n, 128), t256 = tm * ceil_div(p.n, 256);
   B2E_CHECK(t128 <= 0x3fffffffLL, kErrInvalid, "fp8_linear: too many tiles");
   // Tiles of 128 features run two CTAs an SM; tiles of 256 read less shared memory

@@ -154,6 +154,8 @@ def linear_ref(q, scale, wq, wscale, bias, relu):
     (5, 17000, 136, False, False, torch.float32), (40, 40000, 20000, False, False, torch.bfloat16), (2500, 512, 2050, True, False, torch.float16),
     # whole tiles and halves in one launch, the last half empty or whole; whole tiles only
     (3845, 200, 1290, True, False, torch.float32), (4200, 300, 1280, True, True, torch.bfloat16), (3845, 2100, 1000, False, False, torch.float16),
+    # blocks of 64 rows with the groups shared out over a cluster
+    (65, 2048, 1280, True, False, torch.bfloat16), (400, 4100, 250, True, True, torch.float32), (200, 8192, 128, False, False, torch.float16),
 ])
 def test_fp8_linear(m, k, n, bias, relu, out):
     """A product's terms are exact in float32; a group's 128 are summed in 4 steps and the groups one
