@@ -26,16 +26,20 @@
 // blocks of 32 tokens do not touch, and the exponential of the difference inside
 // the diagonal blocks, so nothing overflows for decays below one.
 //
-// Sixteen warps: 0 TMA loads; 1 issues the MMAs; 2-3 the decays of one head each
-// (and zeros behind a sequence's end); 4-7 S from G; 8-11 the state: its decay,
-// its bf16 copy and the split operand; 12-15 y: exp(c) on C H^T, skip, gate and
-// stores. The chain of a chunk is state ready -> C H^T -> scaled -> + S X -> y;
-// the state's products, G of the next chunk and the elementwise work of the other
-// warps run beside it.
+// Twenty-eight warps: 0 TMA loads; 1 the state's MMAs; 2 the decays, a half-warp a
+// head (and zeros behind a sequence's end); 3 the MMAs of G and y; 4-11 S from G;
+// 12-19 the state: its decay, its bf16 copy and the split operand; 20-27 y: exp(c)
+// on C H^T, skip, gate and stores. The chain of a chunk is state ready -> C H^T ->
+// scaled -> + S X -> y; the state's products, G of the next chunk, decays up to
+// three chunks ahead and the gate run beside it. There are two MMA issuers because
+// the state's chain must not queue behind y's.
 //
-// What bounds it: instruction issue (the elementwise work of 2 x 128 x 64 values
-// of x, y, z and 2 x 128 x 128 pairs) and HBM are close; the tensor cores need
-// 6 x 128 x 128 x 128 products a chunk and pair.
+// What bounds it: the handoffs along that chain and instruction latency (seven
+// warps a scheduler issue about every other cycle); the tensor cores need 6 x 128
+// x 128 x 128 products a chunk and pair, and HBM less. 37 sequences of 4096
+// tokens, 16 heads, state 128: 443 us with the gate, 350 without (755 and 608 with
+// sixteen warps and one MMA issuer); 64 sequences of 512 tokens, 64 heads: 530 us;
+// one chunk alone 18 us.
 #include <algorithm>
 
 #include "packed.cuh"
@@ -890,8 +894,14 @@ void run(const ScanParams& p, int seg, cudaStream_t s) {
 
 }  // namespace
 
+// A chunk costs this kernel the same for 1 token as for 128, the recurrence kernel
+// by the token. While all CTAs run at once the longest sequence decides: 4
+// sequences, 8 heads, of 16, 24, 32 tokens take 14.5 us here, 12.1, 16.4, 20.1
+// there. Beyond that the mean does: 256 sequences of 16, 20, 24 tokens take 99 us
+// here, 84, 104, 115 there.
 bool scan_tc_eligible(const ScanParams& p) {
-  return p.type == kBF16 && p.size == 64 && (p.state == 64 || p.state == 128) && p.plan.longest >= 32 && aligned(p.x, 16) &&
+  const bool long_enough = (long long)p.plan.seqs * ((p.heads + 1) / 2) <= 148 ? p.plan.longest >= 24 : p.plan.tokens >= 20LL * p.plan.seqs;
+  return long_enough && p.type == kBF16 && p.size == 64 && (p.state == 64 || p.state == 128) && aligned(p.x, 16) &&
          aligned(p.b, 16) && aligned(p.c, 16) && aligned(p.y, 32) && p.ldx % 8 == 0 && p.ldb % 8 == 0 && p.ldc % 8 == 0 &&
          p.ldy % 16 == 0 && (!p.z || (aligned(p.z, 32) && p.ldz % 16 == 0));
 }
