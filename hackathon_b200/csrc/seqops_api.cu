@@ -207,6 +207,7 @@ int b2e_mamba2_scan(const b2e_sequences* plan, const b2e_scan_args* args, void* 
     p.work = work;
     p.work_bytes = work ? size_t(work_bytes < 0 ? 0 : work_bytes) : 0;
     B2E_CHECK(p.work_bytes >= scan_workspace(p), kErrInvalid, "mamba2_scan: the workspace is too small");
+    B2E_CHECK((reinterpret_cast<uintptr_t>(work) & 15) == 0, kErrInvalid, "mamba2_scan: the workspace starts on a 16-byte boundary");
     p.err = seqops_error_word();
     mamba2_scan(p, static_cast<cudaStream_t>(stream));
   });

@@ -445,6 +445,10 @@ def mamba2_scan(ssm, x, b, c, dt, a, seqs: Optional[SequenceBatch] = None, d=Non
     (rows, heads), ``a`` and ``d`` (heads,) float32. The state and all sums are float32 and y
     is rounded once to x's type. Without ``seqs`` each row is one token of that row of
     ``ssm``, as in ``mamba2_step``. Rows behind the batch's tokens are not read and give zeros.
+
+    A value that is not finite stays in its own sequence and reaches no earlier token; of x, it
+    makes its row's y NaN from its token on. ``a`` is meant to be at most zero: with one above,
+    bf16 prompts (chunks of 128 tokens) overflow where the sum of a t over a chunk passes 88.
     """
     _scan_state_ok(ssm)
     nrows, h, p, n = ssm.shape

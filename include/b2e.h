@@ -288,7 +288,10 @@ B2E_API int b2e_causal_conv(const b2e_sequences* plan, float* window, const void
  * have rows of heads * size values, b and c of state (1..256), dt of heads
  * float32; d and z may be NULL. Long sequences in a small batch are split over
  * the device, which takes b2e_mamba2_scan_workspace() bytes (16-byte aligned, 0
- * and NULL where none is needed) for the same plan and arguments. y may not overlap an input. */
+ * and NULL where none is needed) for the same plan and arguments. y may not overlap an
+ * input. a is meant to be at most 0: above, prompts in bf16 (chunks of 128 tokens) overflow
+ * where the sum of a t over a chunk passes 88. A value of x that is not finite makes its
+ * row's y NaN from its token on. */
 typedef struct b2e_scan_args {
   float* ssm;
   const void* x;

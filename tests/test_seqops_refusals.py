@@ -161,14 +161,15 @@ def test_c_abi_refuses_before_any_device_call():
     ]:
         rc, msg = call("b2e_causal_conv", p, P, P, 0, 8, rows, 8, P, None, taps, 0, P, 8, None)
         assert rc == -1 and match in msg
-    def scan(p=None, work=0, **kw):
+    def scan(p=None, work=0, at=None, **kw):
         a = dict(ssm=P, x=P, b=P, c=P, dt=P, a=P, d=None, z=None, y=P, ldx=32, ldb=16, ldc=16, lddt=4, ldz=0, ldy=32, rows=5,
                  heads=4, size=8, state=16, dtype=0, softplus=1)
-        return call("b2e_mamba2_scan", p or plan(), C.byref(_lib.ScanArgsC(**{**a, **kw})), None, work, None)
+        return call("b2e_mamba2_scan", p or plan(), C.byref(_lib.ScanArgsC(**{**a, **kw})), at, work, None)
     for kw, match in [
         (dict(state=257), "1..256"), (dict(heads=0), "positive"), (dict(dtype=3), "unknown dtype"), (dict(x=None), "null"),
         (dict(ldx=31), "row stride"), (dict(ssm=P + 4), "16-byte"), (dict(rows=4), "more tokens"),
         (dict(p=plan(tokens=5000, longest=5000, seqs=1), rows=5000), "workspace"),
+        (dict(p=plan(tokens=5000, longest=5000, seqs=1), rows=5000, at=P + 8, work=1 << 40), "workspace starts"),
     ]:
         rc, msg = scan(**kw)
         assert rc == -1 and match in msg, (kw, rc, msg)
