@@ -24,7 +24,7 @@
 //    features, N = BR rows (16, 32 or 64; a grid of them above 64); the groups are
 //    shared out over a cluster of up to 8 CTAs, whose float32 sums meet through
 //    distributed shared memory in rank order (the same result every time). Bound
-//    by latency at the sizes it is for: 1 x 2048 x 8448 takes 7.6 us, 2.7 of them
+//    by latency at the sizes it is for: 1 x 2048 x 8448 takes 7.3 us, 2.7 of them
 //    its weight's bytes, the rest the first load, the joining and the launch.
 #include <algorithm>
 #include <cooperative_groups.h>
@@ -361,12 +361,13 @@ __global__ void __launch_bounds__(RowsCfg<BN>::THREADS, RowsCfg<BN>::CTAS)
 // --------------------------------------------------------- few-rows kernel
 
 constexpr int kFewStages = 4;  // 8, one CTA an SM, left clusters to a second round: 1 x 16384 x 2048 21.5 us against 12.4
+constexpr int kFewBufs = 4;  // accumulators in TMEM, so that the MMAs need not wait for each one's reading: 3% to 5% over two
 constexpr int kFewThreads = 64 + 128, kFewSplit = 8;  // CTAs of a cluster at most
 
 template <int BR>
 struct FewCfg {
   static constexpr uint32_t TILE_W = 128 * kKB, TILE_X = BR * kKB, STAGE = TILE_W + TILE_X;
-  static constexpr uint32_t TMEM = 2 * BR < 32 ? 32 : 2 * BR;
+  static constexpr uint32_t TMEM = kFewBufs * BR;
   // the ring; the float32 sums of the CTA's tile reuse it; then the row scales
   static size_t smem(int stages, int local_groups) {
     return 1024 + size_t(std::max(stages * int(STAGE), 128 * BR * 4)) + size_t(local_groups) * BR * 4 + 512;
@@ -388,8 +389,8 @@ __global__ void __launch_bounds__(kFewThreads)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring + size_t(per) * BR * 4);
   uint64_t* empty = full + kFewStages;
   uint64_t* pfull = empty + kFewStages;
-  uint64_t* pempty = pfull + 2;
-  uint64_t* done = pempty + 2;
+  uint64_t* pempty = pfull + kFewBufs;
+  uint64_t* done = pempty + kFewBufs;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -398,7 +399,7 @@ __global__ void __launch_bounds__(kFewThreads)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kFewBufs; ++b) {
       mbar_init(&pfull[b], 1);
       mbar_init(&pempty[b], 4);
     }
@@ -442,8 +443,8 @@ __global__ void __launch_bounds__(kFewThreads)
     const uint64_t dw0 = tc::desc_k(smem_u32(smem)), dx0 = tc::desc_k(smem_u32(smem) + K::TILE_W);
 #pragma unroll 1
     for (int it = 0; it < ng; ++it) {
-      const int s = it % stages, b = it & 1;
-      bool ok = (it < 2 || mbar_wait(&pempty[b], ((it >> 1) & 1) ^ 1, abort_flag)) && mbar_wait(&full[s], (it / stages) & 1, abort_flag);
+      const int s = it % stages, b = it % kFewBufs;
+      bool ok = (it < kFewBufs || mbar_wait(&pempty[b], ((it / kFewBufs) & 1) ^ 1, abort_flag)) && mbar_wait(&full[s], (it / stages) & 1, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0 && !*abort_flag) atomicExch(e.err, kFp8TimeoutMma);
         *abort_flag = 1;
@@ -466,18 +467,16 @@ __global__ void __launch_bounds__(kFewThreads)
     mbar_wait(done, 0, &never);
   } else {
     const int q = warp & 3, tid = threadIdx.x - 64;
-    // the scales of this CTA's rows and groups, while the first tiles arrive
+    // the products of scales of this CTA's rows and groups, while the first tiles arrive
+    const float* ws = e.ws + (long long)(n0 / kFp8Group) * e.wgroups + g0;
     for (int i = tid; i < ng * BR; i += 128) {
       const int r = m0 + i % BR;
-      xsc[i] = r < e.m ? e.xs[(long long)r * e.groups + g0 + i / BR] : 0.f;
+      xsc[i] = r < e.m ? ws[i / BR] * e.xs[(long long)r * e.groups + g0 + i / BR] : 0.f;
     }
     named_bar(1, 128);
-    const float* ws = e.ws + (long long)(n0 / kFp8Group) * e.wgroups + g0;
-    float w = ng > 0 ? ws[0] : 0.f;
     for (int it = 0; it < ng; ++it) {
-      const int b = it & 1;
-      const float wn = it + 1 < ng ? ws[it + 1] : 0.f;
-      const bool ok = mbar_wait(&pfull[b], (it >> 1) & 1, abort_flag);
+      const int b = it % kFewBufs;
+      const bool ok = mbar_wait(&pfull[b], (it / kFewBufs) & 1, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0 && !*abort_flag) atomicExch(e.err, kFp8TimeoutEpi);
         *abort_flag = 1;
@@ -498,13 +497,12 @@ __global__ void __launch_bounds__(kFewThreads)
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const float4 x4 = *reinterpret_cast<const float4*>(xsc + it * BR + j + i);
-          acc[j + i] = fmaf(__uint_as_float(r[i]), w * x4.x, acc[j + i]);
-          acc[j + i + 1] = fmaf(__uint_as_float(r[i + 1]), w * x4.y, acc[j + i + 1]);
-          acc[j + i + 2] = fmaf(__uint_as_float(r[i + 2]), w * x4.z, acc[j + i + 2]);
-          acc[j + i + 3] = fmaf(__uint_as_float(r[i + 3]), w * x4.w, acc[j + i + 3]);
+          acc[j + i] = fmaf(__uint_as_float(r[i]), x4.x, acc[j + i]);
+          acc[j + i + 1] = fmaf(__uint_as_float(r[i + 1]), x4.y, acc[j + i + 1]);
+          acc[j + i + 2] = fmaf(__uint_as_float(r[i + 2]), x4.z, acc[j + i + 2]);
+          acc[j + i + 3] = fmaf(__uint_as_float(r[i + 3]), x4.w, acc[j + i + 3]);
         }
       }
-      w = wn;
     }
   }
   tc::fence_before();
@@ -583,8 +581,8 @@ void launch_rows(const Fp8GemmParams& p, const Args& e, cudaStream_t s) {
 // False where the rows kernel takes less time. With one round of tiles over the SMs
 // that kernel takes 3 + 0.385 us a group, and this one 4 (one row) to 5.4 (64 rows)
 // + 0.5 us a group of its share, which is the comparison below. Rows against few:
-// 1 x 256 x 1280 3.8 / 4.2 us, 1 x 2048 x 8448 9.4 / 7.6, 64 x 2048 x 8448 9.7 /
-// 10.6, 64 x 4096 x 1024 15.5 / 7.3, 400 x 4096 x 1024 16.1 / 14.8, 1000 x 4096 x
+// 1 x 256 x 1280 3.8 / 4.2 us, 1 x 2048 x 8448 9.4 / 7.3, 64 x 2048 x 8448 9.7 /
+// 10.5, 64 x 4096 x 1024 15.5 / 7.3, 400 x 4096 x 1024 16.1 / 13.9, 1000 x 4096 x
 // 1024 16.7 / 25.4, 1 x 4096 x 40000 (more than L2) 42.4 / 43.4.
 // False too where the scales of a CTA's groups would not fit beside the ring.
 template <int BR>

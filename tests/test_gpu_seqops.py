@@ -173,13 +173,13 @@ def test_fp8_linear(m, k, n, bias, relu, out):
     assert K.device_error() == 0
 
 
-@pytest.mark.parametrize("m", [4, 200])
-def test_fp8_linear_rows_keep_to_themselves(m):
+@pytest.mark.parametrize("m,k", [(4, 300), (200, 300), (4, 1500), (100, 1500)])
+def test_fp8_linear_rows_keep_to_themselves(m, k):
     """A row with a NaN, an infinite scale or a zero scale leaves the other rows' bits alone; strided and
     unaligned operands give the packed ones' bits."""
     g = gen(m)
-    q, scale = K.quantize_fp8(rnd(g, m, 300))
-    wq, wscale = K.quantize_fp8_weight(rnd(g, 140, 300))
+    q, scale = K.quantize_fp8(rnd(g, m, k))
+    wq, wscale = K.quantize_fp8_weight(rnd(g, 140, k))
     y = K.fp8_linear(q, scale, wq, wscale)
     bad_q, bad_s = q.clone(), scale.clone()
     bad_q.view(torch.uint8)[1, 5] = 0x7F  # e4m3 NaN
@@ -188,7 +188,7 @@ def test_fp8_linear_rows_keep_to_themselves(m):
     assert z[1].isnan().all() and not z[2].isfinite().any()
     keep = [i for i in range(m) if i not in (1, 2)]
     assert torch.equal(z[keep], y[keep])
-    odd = torch.empty(m, 301, dtype=torch.uint8, device=DEV)[:, 1:]
+    odd = torch.empty(m, k + 1, dtype=torch.uint8, device=DEV)[:, 1:]
     odd.copy_(q.view(torch.uint8) if q.is_contiguous() else q.contiguous().view(torch.uint8))
     assert torch.equal(K.fp8_linear(odd.view(torch.float8_e4m3fn), scale, wq, wscale), y)
     assert torch.equal(K.fp8_linear(q, scale.T.contiguous().T, wq, wscale), y)
