@@ -27,12 +27,12 @@
 // the diagonal blocks, so nothing overflows for decays below one.
 //
 // Twenty-eight warps: 0 TMA loads; 1 the state's MMAs; 2 the decays, a half-warp a
-// head (and zeros behind a sequence's end); 3 the MMAs of G and y; 4-11 S from G;
-// 12-19 the state: its decay, its bf16 copy and the split operand; 20-27 y: exp(c)
-// on C H^T, skip, gate and stores. The chain of a chunk is state ready -> C H^T ->
-// scaled -> + S X -> y; the state's products, G of the next chunk, decays up to
-// three chunks ahead and the gate run beside it. There are two MMA issuers because
-// the state's chain must not queue behind y's.
+// head; 3 the MMAs of G and y (and zeros in B behind a sequence's end); 4-11 S from
+// G; 12-19 the state: its decay, its bf16 copy, the split operand (and zeros in x
+// behind the end); 20-27 y: exp(c) on C H^T, skip, gate and stores. The chain of a
+// chunk is state ready -> C H^T -> scaled -> + S X -> y; the state's products, G of
+// the next chunk, decays up to three chunks ahead and the gate run beside it. There
+// are two MMA issuers because the state's chain must not queue behind y's.
 //
 // What bounds it: the handoffs along that chain and instruction latency (seven
 // warps a scheduler issue about every other cycle); the tensor cores need 6 x 128
@@ -225,8 +225,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + K::oBar);
   uint64_t *cbfull = bar, *cbempty = bar + 2, *xfull = bar + 4, *xempty = bar + 7, *vfull = bar + 10, *vempty = bar + 13,
            *xwfull = bar + 16, *xwempty = bar + 18, *xscan = bar + 20, *gfull = bar + 23, *sfull = bar + 24, *y2full = bar + 25,
-           *y2scaled = bar + 26, *yfull = bar + 27, *yfree = bar + 28, *hready = bar + 29, *hdone = bar + 30, *done = bar + 31;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 32);
+           *y2scaled = bar + 26, *yfull = bar + 27, *yfree = bar + 28, *hready = bar + 29, *hdone = bar + 30, *done = bar + 31,
+           *bzero = bar + 32;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 33);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -253,6 +254,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(hready, 8);
     mbar_init(hdone, 1);
     mbar_init(done, ENDS ? 1 : 2);
+    mbar_init(bzero, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
@@ -335,6 +337,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int st = c & 1;
       const uint64_t dB = desc_mn(sbase + st * K::STAGE + K::oB, kTile);
       if (!(ok = wait(hready, c & 1) && wait(&cbfull[st], (c >> 1) & 1))) break;
+      if (end - t.first - c * Q < Q && !(ok = wait(bzero, 0))) break;  // the last chunk's, a short one
 #pragma unroll 1
       for (int j = 0; j < 4; ++j) {
         if (!(ok = wait(&xwfull[j & 1], j >> 1))) break;
@@ -419,6 +422,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc::commit(gfull);
           }
           __syncwarp();
+          const int valid = end - t.first - i * Q;
+          if (valid < Q) {
+            // Behind the sequence's end lie other sequences' rows of B: zeros before the
+            // state's products, so that nothing of them meets one (G's columns there
+            // are masked in S, and the state's warps do the same for x). Here, because
+            // this warp takes every phase of these barriers in turn: a parity cannot
+            // tell a phase from the one two before it.
+            if (!(ok = wait(gfull, i & 1))) break;
+            uint8_t* bt = smem + (i & 1) * K::STAGE + K::oB;
+#pragma unroll 4
+            for (int k = valid * 8 + lane; k < Q * 8; k += 32)
+#pragma unroll
+              for (int n = 0; n < NB; ++n) *reinterpret_cast<uint4*>(bt + n * kTile + k * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async();
+            arrive(bzero);
+          }
         }
       }
       if (tc::elect()) tc::commit(done);
@@ -442,7 +461,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     Turn vt(kVecs);
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c, vt.next()) {
-      const int st = c & 1, vs = vt.at, valid = min(Q, end - t.first - c * Q);
+      const int vs = vt.at, valid = min(Q, end - t.first - c * Q);
       Pair cum[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -494,24 +513,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (l == 0) v.total = ex2(total.hi + total.lo);
       at += Q * p.lddt;
       fetch(end - t.first - (c + 1) * Q);
-      if (valid < Q) {
-        // Behind the sequence's end lie other sequences' rows: zeros, so that
-        // nothing of them meets a product.
-        ok = wait(&cbfull[st], (c >> 1) & 1);
-        Turn xt(kXSlots, 2 * c);
-#pragma unroll 1
-        for (int h = 0; h < 2 && ok; ++h, xt.next()) {
-          if (!(ok = wait(&xfull[xt.at], xt.phase))) break;
-          uint4* xr = reinterpret_cast<uint4*>(smem + K::oX + xt.at * kTile);
-          for (int i = valid * 8 + lane; i < Q * 8; i += 32) xr[i] = make_uint4(0, 0, 0, 0);
-        }
-        if (!ok) break;
-        for (int n = 0; n < NB; ++n) {
-          uint4* br = reinterpret_cast<uint4*>(smem + st * K::STAGE + K::oB + n * kTile);
-          for (int i = valid * 8 + lane; i < Q * 8; i += 32) br[i] = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async();
-      }
       arrive(&vfull[vt.at]);
     }
     if (!ok && lane == 0) failed();
@@ -652,7 +653,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       arrive(hready);
       // exp(c[T] - c[s]) dt[s] x[s], split over three bf16 values, tokens along the columns
       if (!(ok = wait(&xfull[sl], xt.phase))) break;
-      const uint8_t* xs = smem + K::oX + sl * kTile + (pr & 7) * 2;
+      uint8_t* xs = smem + K::oX + sl * kTile + (pr & 7) * 2;
+      const int valid = end - t.first - c * Q;
+      if (valid < Q) {  // behind the sequence's end: zeros (the warp's 32 rows, four 16-byte vectors of a token, and its half's tokens)
+#pragma unroll 1
+        for (int i = lane; i < Q / 2 * 4; i += 32) {
+          const int s = (i >> 7) * 64 + half * 32 + ((i >> 2) & 31), v16 = (q & 1) * 4 + (i & 3);
+          if (s >= valid) *reinterpret_cast<uint4*>(smem + K::oX + sl * kTile + s * 128 + ((v16 ^ (s & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+        __syncwarp();
+      }
       F2 finite = f2(0.f, 0.f);
       const F2 zero = finite, minus = f2(-1.f, -1.f);
 #pragma unroll 1
@@ -704,7 +715,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 1
           for (int s = Q - 1; s >= 0; --s) {
             if (((s >> 5) & 1) != half) continue;
-            uint16_t* e = reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(xs) + s * 128 + (((pr >> 3) ^ (s & 7)) << 4));
+            uint16_t* e = reinterpret_cast<uint16_t*>(xs + s * 128 + (((pr >> 3) ^ (s & 7)) << 4));
             if ((*e & 0x7f80) == 0x7f80) {
               first = s;
               *e = 0;
