@@ -163,11 +163,11 @@ __global__ void __launch_bounds__(32 * kConvWarps) k_conv(const ConvParams p, in
   const int tile = int(gw / vblocks), lane = threadIdx.x & 31;
   const int c = (int(gw % vblocks) * 32 + lane) * VC;
   const SeqTile t = seq_tile(p.plan, tile, len);
-  if (!t.live && p.err && t.start < t.end && (t.start < 0 || t.end > p.plan.tokens)) *p.err = 1;
+  if (lane == 31 && gw % vblocks == 0) seq_report(p.plan, tile, false, p.err);
   if (!t.live || c >= p.channels) return;
   const int slot = p.plan.slots ? p.plan.slots[t.seq] : t.seq;
   if (slot < 0 || slot >= p.plan.state_rows) {
-    if (p.err) *p.err = 1;
+    *p.err = 1;
     return;
   }
   const int end = min(t.end, t.first + len);
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(32 * kConvWarps) k_conv_step(const ConvParams 
       slot = p.plan.slots ? p.plan.slots[s] : s;
       if (slot < 0 || slot >= p.plan.state_rows) {
         slot = -1;
-        if (p.err) *p.err = 1;
+        *p.err = 1;
       }
     }
     at[i] = slot < 0 ? -1 : ((long long)slot * p.channels + c) * W;

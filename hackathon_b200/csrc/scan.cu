@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(128) k_scan_step(const ScanParams p) {
   const int seq = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
   const int slot = p.plan.slots ? p.plan.slots[seq] : seq;
   if (slot < 0 || slot >= p.plan.state_rows) {
-    if (threadIdx.x == 0 && p.err) *p.err = 1;
+    if (threadIdx.x == 0) *p.err = 1;
     return;
   }
   const int lane = threadIdx.x & 31, c0 = lane % LPR, nv = p.state / 4;
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(256) k_scan_step_any(const ScanParams p) {
   const int seq = blockIdx.x / p.heads, h = blockIdx.x % p.heads, lane = threadIdx.x & 31;
   const int slot = p.plan.slots ? p.plan.slots[seq] : seq;
   if (slot < 0 || slot >= p.plan.state_rows) {
-    if (threadIdx.x == 0 && p.err) *p.err = 1;
+    if (threadIdx.x == 0) *p.err = 1;
     return;
   }
   const float dtr = p.dt[seq * p.lddt + h];
@@ -199,10 +199,11 @@ __global__ void __launch_bounds__(128) k_scan_seq(const ScanParams p, ScanWork w
   } else {
     t = seq_whole(p.plan, tile);
   }
+  if (threadIdx.x == 127 && h == 0 && p0 == 0) seq_report(p.plan, tile, seg == 0, p.err);
   if (!t.live) return;
   const int slot = p.plan.slots ? p.plan.slots[t.seq] : t.seq;
   if (slot < 0 || slot >= p.plan.state_rows) {
-    if (threadIdx.x == 0 && p.err) *p.err = 1;
+    if (threadIdx.x == 0) *p.err = 1;
     return;
   }
   const int end = seg > 0 ? min(t.end, t.first + seg) : t.end;

@@ -187,10 +187,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else {
     t = seq_whole(p.plan, tile);
   }
+  if (threadIdx.x == kTcThreads - 1 && h0 == 0) seq_report(p.plan, tile, g.seg == 0, p.err);
   if (!t.live) return;
   const int slot = p.plan.slots ? p.plan.slots[t.seq] : t.seq;
   if (slot < 0 || slot >= p.plan.state_rows) {
-    if (threadIdx.x == 0 && p.err) *p.err = 1;
+    if (threadIdx.x == 0) *p.err = 1;
     return;
   }
   const int end = g.seg > 0 ? min(t.end, t.first + g.seg) : t.end;

@@ -170,4 +170,14 @@ __device__ __forceinline__ SeqTile seq_whole(const SeqPlan& p, int i) {
   return t;
 }
 
+// Reports a plan whose entries leave its operands: tile i of a launch that covers
+// every sequence (there are at least as many tiles) answers for sequence i, whatever
+// tile i itself works on, because bad starts can hide a sequence from the search.
+// `whole`: the launch goes by `order`. One thread a tile.
+__device__ __forceinline__ void seq_report(const SeqPlan& p, int tile, bool whole, int* err) {
+  if (tile >= p.seqs) return;
+  const int s = p.starts[tile], e = p.starts[tile + 1], o = whole && p.order ? p.order[tile] : 0;
+  if (s < 0 || e < s || e > p.tokens || o < 0 || o >= p.seqs) *err = 1;
+}
+
 }  // namespace b2e

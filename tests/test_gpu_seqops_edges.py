@@ -1,9 +1,12 @@
 """The run-of-tokens operators where their contract is easily broken: sequence ends inside a
 chunk, plans and extents at their limits, values at the ends of their types."""
 
+import ctypes as C
+
 import pytest
 import torch
 
+from hackathon_b200 import _lib as L
 from hackathon_b200 import kernels as K
 from tests import seqops_ref as R
 from tests.test_gpu_seqops import DEV, PAIRS, TYPES, gen, ids, rnd, scan_inputs
@@ -59,3 +62,117 @@ def test_scan_ends_inside_a_chunk(dt, h, n, gate):
     cut = {k: clean[k][:few] if k in names else clean[k] for k in clean}
     cut["ssm"] = clean["ssm"][:8]
     against_recurrence(cut, before[:8], y[:few], lengths[:8], PAIRS[dt])
+
+
+# ------------------------------------------------- plans that leave their operands
+
+
+def c_plan(starts, slots, order, tokens, state_rows, longest):
+    """A plan as a C host makes it (it keeps the device arrays that it points into)."""
+    arrays = [None if v is None else torch.tensor(v, dtype=torch.int32, device=DEV) for v in (starts, slots, order)]
+    seqs = len(starts) - 1 if starts is not None else len(slots)
+    plan = L.SequencesC(*[None if a is None else a.data_ptr() for a in arrays], seqs, tokens, state_rows, longest)
+    plan.arrays = arrays
+    return plan
+
+
+def c_scan(inp, plan):
+    _, h, p, n = inp["ssm"].shape
+    y = torch.zeros_like(inp["x"])
+    at = {k: inp[k].data_ptr() for k in ("ssm", "x", "b", "c", "dt", "a")}
+    args = L.ScanArgsC(**at, y=y.data_ptr(), ldx=h * p, ldb=n, ldc=n, lddt=h, ldy=h * p, rows=len(y), heads=h, size=p, state=n,
+                       dtype=K._TORCH_DTYPES[y.dtype], softplus=1)
+    need = C.c_int64()
+    L.check(L.lib().b2e_mamba2_scan_workspace(C.byref(plan), C.byref(args), C.byref(need)))
+    work = torch.empty(max(need.value, 1), dtype=torch.uint8, device=DEV)
+    L.check(L.lib().b2e_mamba2_scan(C.byref(plan), C.byref(args), work.data_ptr(), need.value, None))
+    torch.cuda.synchronize()
+    return y
+
+
+def c_conv(window, x, w, plan):
+    y = torch.zeros_like(x)
+    L.check(L.lib().b2e_causal_conv(C.byref(plan), window.data_ptr(), x.data_ptr(), K._TORCH_DTYPES[x.dtype], x.shape[1], len(x),
+                                    x.shape[1], w.data_ptr(), None, 4, 0, y.data_ptr(), x.shape[1], None))
+    torch.cuda.synchronize()
+    return y
+
+
+def reported():
+    """The error word says that a plan was out of range, once: reading clears it."""
+    return K.device_error() == 1 and K.device_error() == 0
+
+
+# three sequences: what is wrong, and those that are still stepped
+BAD_PLANS = [
+    (dict(starts=[0, 40, 70, 140]), [0, 1]), (dict(starts=[-8, 40, 70, 100]), [1, 2]), (dict(starts=[0, 40, 30, 100]), []),
+    (dict(starts=[0, 40, 2 ** 31 - 1, 100]), [0]), (dict(starts=[0, -2 ** 31, 70, 100]), [2]),
+    (dict(slots=[0, 3, 2]), [0, 2]), (dict(slots=[0, 1, -1]), [0, 1]), (dict(slots=[-2 ** 31, 2 ** 31 - 1, 2]), [2]),
+    (dict(order=[2, 1, 3]), [1, 2]), (dict(order=[-1, 0, 1]), [0, 1]),
+]
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("wrong,good", BAD_PLANS, ids=[f"{next(iter(w))}-{i}" for i, (w, _) in enumerate(BAD_PLANS)])
+def test_scan_and_conv_report_a_bad_plan(dt, wrong, good):
+    """The sequence that leaves the operands or the table is not stepped, the others are, and the word says so."""
+    assert K.device_error() == 0
+    spec = dict(starts=[0, 40, 70, 100], slots=[0, 1, 2], order=[2, 0, 1])
+    at = list(zip(spec["starts"], spec["starts"][1:]))
+    inp = scan_inputs(60, 3, 100, 4, 64, 128, dt, False)
+    before, same = inp["ssm"].clone(), {**inp, "ssm": inp["ssm"].clone()}
+    want = c_scan(same, c_plan(**spec, tokens=100, state_rows=3, longest=40))
+    assert K.device_error() == 0
+    plan = c_plan(**{**spec, **wrong}, tokens=100, state_rows=3, longest=40)
+    y = c_scan(inp, plan)
+    assert reported()
+    for i, (s, e) in enumerate(at):
+        if i in good:
+            assert torch.equal(y[s:e], want[s:e]) and torch.equal(inp["ssm"][i], same["ssm"][i])
+        elif "starts" not in wrong:  # (a shared border moves a neighbour's rows too)
+            assert not y[s:e].any() and torch.equal(inp["ssm"][i], before[i])
+
+    if "order" in wrong:  # the convolution does not go by it
+        return
+    x, w = rnd(gen(61), 100, 64).to(dt), rnd(gen(62), 64, 4)
+    win = rnd(gen(63), 3, 64, 3)
+    before, clean = win.clone(), win.clone()
+    want = c_conv(clean, x, w, c_plan(**spec, tokens=100, state_rows=3, longest=40))
+    y = c_conv(win, x, w, plan)
+    assert reported()
+    for i, (s, e) in enumerate(at):
+        if i in good:
+            assert torch.equal(y[s:e], want[s:e]) and torch.equal(win[i], clean[i])
+        elif "starts" not in wrong:
+            assert not y[s:e].any() and torch.equal(win[i], before[i])
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("wrong", [dict(starts=[0, 3000, 3060]), dict(starts=[-5, 2960, 3000]), dict(slots=[2, 1]), dict(starts=[0, 2960, 2000])])
+def test_split_scan_reports_a_bad_plan(dt, wrong):
+    """The same where sequences are split into segments."""
+    inp = scan_inputs(64, 2, 3000, 2, 64, 128, dt, False)
+    before = inp["ssm"].clone()
+    plan = c_plan(**{**dict(starts=[0, 2960, 3000], slots=[0, 1], order=[0, 1]), **wrong}, tokens=3000, state_rows=2, longest=2960)
+    assert K.device_error() == 0
+    c_scan(inp, plan)
+    assert reported()
+    bad = 0 if "slots" in wrong or wrong["starts"][0] < 0 else 1
+    assert torch.equal(inp["ssm"][bad], before[bad]) and not torch.equal(inp["ssm"][1 - bad], before[1 - bad])
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [128, 30])
+def test_single_tokens_report_a_bad_plan(dt, n):
+    inp = scan_inputs(65, 3, 3, 2, 64, n, dt, False)
+    before = inp["ssm"].clone()
+    plan = c_plan(None, [0, 3, 2], None, tokens=3, state_rows=3, longest=1)
+    assert K.device_error() == 0
+    y = c_scan(inp, plan)
+    assert reported()
+    assert torch.equal(inp["ssm"][1], before[1]) and not torch.equal(inp["ssm"][2], before[2]) and not y[1].any() and y[2].any()
+    x, w, win = rnd(gen(66), 3, 64).to(dt), rnd(gen(67), 64, 4), rnd(gen(68), 3, 64, 3)
+    before = win.clone()
+    y = c_conv(win, x, w, plan)
+    assert reported()
+    assert torch.equal(win[1], before[1]) and not torch.equal(win[2], before[2]) and not y[1].any() and y[2].any()
