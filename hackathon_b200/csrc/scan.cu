@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(256) k_scan_join(const ScanParams p, ScanWork 
   const long long hp = (long long)p.size * p.state, e = ((long long)blockIdx.y * blockDim.x + threadIdx.x) * V;
   const int start = p.plan.starts[seq], end = p.plan.starts[seq + 1];
   const int slot = p.plan.slots ? p.plan.slots[seq] : seq;
-  if (e >= hp || start < 0 || end > p.plan.tokens || end - start <= seg || slot < 0 || slot >= p.plan.state_rows) return;
+  if (e >= hp || start < 0 || end > p.plan.tokens || end < start || end - start <= seg || slot < 0 || slot >= p.plan.state_rows) return;
   const int segs = ceil_div(end - start, seg);
   const long long tile0 = start / seg + seq, step = (long long)p.heads * hp;
   const auto load = [](const float* at, float (&v)[V]) {

@@ -148,7 +148,8 @@ def test_scan_and_conv_report_a_bad_plan(dt, wrong, good):
 
 
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
-@pytest.mark.parametrize("wrong", [dict(starts=[0, 3000, 3060]), dict(starts=[-5, 2960, 3000]), dict(slots=[2, 1]), dict(starts=[0, 2960, 2000])])
+@pytest.mark.parametrize("wrong", [dict(starts=[0, 3000, 3060]), dict(starts=[-5, 2960, 3000]), dict(slots=[2, 1]), dict(starts=[0, 2960, 2000]),
+                                   dict(starts=[0, 2960, -2 ** 31])])
 def test_split_scan_reports_a_bad_plan(dt, wrong):
     """The same where sequences are split into segments."""
     inp = scan_inputs(64, 2, 3000, 2, 64, 128, dt, False)
