@@ -211,7 +211,8 @@ __global__ void __launch_bounds__(128) k_scan_seq(const ScanParams p, ScanWork w
   const int lane = threadIdx.x & 31, c16 = lane & 15, rg = threadIdx.x >> 4;
   const long long hp = (long long)p.size * p.state;
   float* own = p.ssm + ((long long)slot * p.heads + h) * hp;
-  float* part = wk.state + ((long long)tile * p.heads + h) * hp;
+  const long long place = seg > 0 ? work_place(wk, p.plan, seg, t.seq, t.start, t.k) : 0;
+  float* part = wk.state + (place * p.heads + h) * hp;
   const float* from = seg > 0 && t.end - t.start > seg ? part : own;
   float* to = ends ? part : own;
   const bool vec = p.state % 4 == 0;  // (the tables then start on 16 bytes)
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(128) k_scan_seq(const ScanParams p, ScanWork w
     }
     if (ASYNC) buf ^= 1;
   }
-  if (ends && threadIdx.x == 0 && p0 == 0) wk.log_decay[(long long)tile * p.heads + h] = logsum;
+  if (ends && threadIdx.x == 0 && p0 == 0) wk.log_decay[place * p.heads + h] = logsum;
   if (ends || end == t.end) {
     scale_state(P);
 #pragma unroll
@@ -413,7 +414,8 @@ __global__ void __launch_bounds__(256) k_scan_join(const ScanParams p, ScanWork 
   const int slot = p.plan.slots ? p.plan.slots[seq] : seq;
   if (e >= hp || start < 0 || end > p.plan.tokens || end < start || end - start <= seg || slot < 0 || slot >= p.plan.state_rows) return;
   const int segs = ceil_div(end - start, seg);
-  const long long tile0 = start / seg + seq, step = (long long)p.heads * hp;
+  const long long zeroth = work_place(wk, p.plan, seg, seq, start, 0) * p.heads + h, rest = work_place(wk, p.plan, seg, seq, start, 1) * p.heads + h;
+  const auto place = [&](int k) { return k > 0 ? rest + (long long)(k - 1) * p.heads : zeroth; };
   const auto load = [](const float* at, float (&v)[V]) {
     if constexpr (V == 4) {
       const float4 a = *reinterpret_cast<const float4*>(at);
@@ -424,24 +426,23 @@ __global__ void __launch_bounds__(256) k_scan_join(const ScanParams p, ScanWork 
   };
   float v[V];
   load(p.ssm + ((long long)slot * p.heads + h) * hp + e, v);
-  float* at = wk.state + (tile0 * p.heads + h) * hp + e;
-  const float* ld = wk.log_decay + tile0 * p.heads + h;
+  float* at = wk.state + e;
   constexpr int U = 4;  // contributions in flight
   for (int k0 = 0; k0 < segs; k0 += U) {
     float c[U][V], g[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (k0 + u + 1 < segs) {
-        load(at + (k0 + u) * step, c[u]);
-        g[u] = ld[(long long)(k0 + u) * p.heads];
+        load(at + place(k0 + u) * hp, c[u]);
+        g[u] = wk.log_decay[place(k0 + u)];
       }
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (k0 + u < segs) {
         if constexpr (V == 4)
-          *reinterpret_cast<float4*>(at + (k0 + u) * step) = make_float4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<float4*>(at + place(k0 + u) * hp) = make_float4(v[0], v[1], v[2], v[3]);
         else
-          at[(k0 + u) * step] = v[0];
+          at[place(k0 + u) * hp] = v[0];
         if (k0 + u + 1 < segs) {
           const float d = expf(g[u]);
 #pragma unroll
@@ -533,8 +534,9 @@ void scan_join(const ScanParams& p, const ScanWork& wk, int seg, cudaStream_t s)
 }
 
 ScanWork scan_work(const ScanParams& p, int seg) {
-  const long long pairs = seq_tiles(p.plan, seg) * p.heads;
+  const long long pairs = work_places(p.plan, seg) * p.heads;
   ScanWork w;
+  w.firsts = std::min(p.plan.seqs, p.plan.tokens / seg);
   w.log_decay = static_cast<float*>(p.work);
   w.state = w.log_decay + (pairs + 63) / 64 * 64;
   return w;
@@ -562,7 +564,7 @@ int scan_segment(const ScanParams& p) {
 size_t scan_workspace(const ScanParams& p) {
   const int seg = scan_segment(p);
   if (seg == 0) return 0;
-  const size_t pairs = size_t(seq_tiles(p.plan, seg)) * p.heads;
+  const size_t pairs = size_t(work_places(p.plan, seg)) * p.heads;
   return ((pairs + 63) / 64 * 64 + pairs * p.size * p.state) * 4;
 }
 

@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int end = g.seg > 0 ? min(t.end, t.first + g.seg) : t.end;
   if (ENDS && end == t.end) return;
   const int chunks = (end - t.first + Q - 1) / Q;
+  const long long place = g.seg > 0 ? work_place(g.wk, p.plan, g.seg, t.seq, t.start, t.k) : 0;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // What the first chunk waits for from HBM, on its way while the CTA sets up: dt,
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int row = (warp & 3) * 32 + lane, half = warp >= 16;
     if (h0 + (row >> 6) < p.heads) {
       const bool joined = g.seg > 0 && t.end - t.start > g.seg;
-      const float* f = (joined ? g.wk.state + ((long long)tile * p.heads + h0) * 64 * N : p.ssm + ((long long)slot * p.heads + h0) * 64 * N) +
+      const float* f = (joined ? g.wk.state + (place * p.heads + h0) * 64 * N : p.ssm + ((long long)slot * p.heads + h0) * 64 * N) +
                        (long long)row * N + half * (N / 2);
 #pragma unroll
       for (int k = 0; k < N / 2; k += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(f + k));
@@ -594,7 +595,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const bool has = head < p.heads;
     const long long hp = 64LL * N;
     float* own = p.ssm + ((long long)slot * p.heads + head) * hp + (long long)pr * N;
-    float* part = g.wk.state + ((long long)tile * p.heads + head) * hp + (long long)pr * N;
+    float* part = g.wk.state + (place * p.heads + head) * hp + (long long)pr * N;
     const float* from = g.seg > 0 && t.end - t.start > g.seg ? part : own;
     uint8_t* hrow = smem + K::oH + prow * 128;
     // the state that the segment starts from, while the first chunk's decays are made
@@ -866,7 +867,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s = add(s, {__shfl_xor_sync(0xffffffffu, s.hi, o), __shfl_xor_sync(0xffffffffu, s.lo, o)});
-      if (lane == 0) g.wk.log_decay[(long long)tile * p.heads + head] = s.hi + s.lo;
+      if (lane == 0) g.wk.log_decay[place * p.heads + head] = s.hi + s.lo;
     }
   }
   tc::fence_before();

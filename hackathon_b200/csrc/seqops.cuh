@@ -108,7 +108,7 @@ struct ScanParams {
   long long ldy;
   int heads, size, state;
   int softplus;
-  void* work;  // scan_workspace() bytes, 256-byte aligned
+  void* work;  // scan_workspace() bytes, 16-byte aligned
   size_t work_bytes;
   int* err;
 };
@@ -130,6 +130,7 @@ __host__ __device__ inline long long seq_tiles(const SeqPlan& p, int len) {
 
 struct SeqTile {
   int seq, start, end, first;  // sequence, its rows [start, end), first row of the tile
+  int k;                       // of the sequence's tiles
   bool live;
 };
 
@@ -153,9 +154,9 @@ __device__ __forceinline__ SeqTile seq_tile(const SeqPlan& p, int tile, int len)
   t.seq = lo;
   t.start = p.starts[lo];
   t.end = p.starts[lo + 1];
-  const int k = tile - (t.start / len + lo);
-  t.first = t.start + k * len;
-  t.live = t.start >= 0 && t.end <= p.tokens && k >= 0 && t.first < t.end;
+  t.k = tile - (t.start / len + lo);
+  t.first = t.start + t.k * len;
+  t.live = t.start >= 0 && t.end <= p.tokens && t.k >= 0 && t.first < t.end;
   return t;
 }
 
@@ -163,6 +164,7 @@ __device__ __forceinline__ SeqTile seq_tile(const SeqPlan& p, int tile, int len)
 __device__ __forceinline__ SeqTile seq_whole(const SeqPlan& p, int i) {
   SeqTile t;
   t.seq = p.order ? p.order[i] : i;
+  t.k = 0;
   t.live = t.seq >= 0 && t.seq < p.seqs;
   t.start = t.first = t.live ? p.starts[t.seq] : 0;
   t.end = t.live ? p.starts[t.seq + 1] : 0;

@@ -177,3 +177,28 @@ def test_single_tokens_report_a_bad_plan(dt, n):
     y = c_conv(win, x, w, plan)
     assert reported()
     assert torch.equal(win[1], before[1]) and not torch.equal(win[2], before[2]) and not y[1].any() and y[2].any()
+
+
+# ------------------------------------------------- split sequences among others
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=ids)
+@pytest.mark.parametrize("lengths", [
+    [1] * 600 + [1500] + [3] * 400 + [0] * 50 + [2300] + [2] * 300,  # far more sequences than segments
+    [384, 384, 129, 300, 257, 1, 128, 640, 256, 1000],               # borders on segments' borders
+    [127] + [1] * 129 + [384, 384, 640, 129, 257, 300] + [0, 1] * 40,
+], ids=["many", "borders", "both"])
+def test_split_sequences_among_others(dt, lengths):
+    """Segments of several split sequences and short ones beside them: each finds its own states."""
+    h = 2
+    slots = torch.randperm(len(lengths), generator=torch.Generator().manual_seed(7)).tolist()
+    inp = scan_inputs(70, len(lengths), sum(lengths), h, 64, 128, dt, True)
+    before = inp["ssm"].clone()
+    plan = K.SequenceBatch(lengths, slots, device=DEV)
+    assert max(lengths) > 256  # where sequences of this batch are split
+    y = scan(inp, plan)
+    want, ssm, ymag, smag = R.scan(before, inp["x"], inp["b"], inp["c"], inp["dt"], inp["a"], lengths, slots, inp["d"], inp["z"])
+    steps = max(lengths) + 1
+    R.close(y, want, R.scan_tol(want, ymag, steps, dt, PAIRS[dt]) + 4 * 2.0 ** -22 * want.abs(), "y")
+    R.close(inp["ssm"], ssm, R.scan_tol(ssm, smag, steps, torch.float32), "ssm")
+    assert K.device_error() == 0
