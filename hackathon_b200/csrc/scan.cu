@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(128) k_scan_seq(const ScanParams p, ScanWork w
     if (threadIdx.x == 0) *p.err = 1;
     return;
   }
-  const int end = seg > 0 ? min(t.end, t.first + seg) : t.end;
+  const int end = seg > 0 && t.end - t.first > seg ? t.first + seg : t.end;
   if (ends && end == t.end) return;
   const int lane = threadIdx.x & 31, c16 = lane & 15, rg = threadIdx.x >> 4;
   const long long hp = (long long)p.size * p.state;

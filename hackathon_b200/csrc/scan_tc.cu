@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (threadIdx.x == 0) *p.err = 1;
     return;
   }
-  const int end = g.seg > 0 ? min(t.end, t.first + g.seg) : t.end;
+  const int end = g.seg > 0 && t.end - t.first > g.seg ? t.first + g.seg : t.end;
   if (ENDS && end == t.end) return;
   const int chunks = (end - t.first + Q - 1) / Q;
   const long long place = g.seg > 0 ? work_place(g.wk, p.plan, g.seg, t.seq, t.start, t.k) : 0;

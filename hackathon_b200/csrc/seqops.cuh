@@ -6,6 +6,10 @@
 
 namespace b2e {
 
+// Rows, columns, tokens and channels of a call: indices are 32-bit (offsets are not),
+// and a tile's or a block's last ones may lie behind the end.
+constexpr int kMaxExtent = 0x7fffffff - 1023;
+constexpr int kMaxSeqs = 1 << 30;
 constexpr int kFp8Group = 128;        // values of a row (rows x columns of a weight block) that share a scale
 constexpr float kFp8Max = 448.0f;     // largest finite e4m3 value
 constexpr float kFp8MinScale = 7.888609052210118e-31f;  // 2^-100: an all-zero group keeps a finite reciprocal
@@ -155,8 +159,9 @@ __device__ __forceinline__ SeqTile seq_tile(const SeqPlan& p, int tile, int len)
   t.start = p.starts[lo];
   t.end = p.starts[lo + 1];
   t.k = tile - (t.start / len + lo);
-  t.first = t.start + t.k * len;
-  t.live = t.start >= 0 && t.end <= p.tokens && t.k >= 0 && t.first < t.end;
+  const long long first = t.start + (long long)t.k * len;
+  t.first = int(first);
+  t.live = t.start >= 0 && t.end <= p.tokens && t.k >= 0 && first < t.end;
   return t;
 }
 

@@ -1,6 +1,7 @@
 // C ABI of the prompt-side operators (include/b2e.h): argument checks, then the
 // launchers of norm_fp8.cu, fp8_gemm.cu, conv.cu and scan.cu.
 #include <functional>
+#include <initializer_list>
 #include <mutex>
 
 #include "../../include/b2e.h"
@@ -22,16 +23,23 @@ constexpr int kMaxDevices = 64;
 std::mutex g_mu;
 int* g_err_ptr[kMaxDevices] = {};
 
+// Every size within the 32-bit indices of the kernels.
+void check_extents(std::initializer_list<long long> sizes) {
+  for (const long long n : sizes) B2E_CHECK(n <= kMaxExtent, kErrInvalid, "sizes are at most 2^31 - 1024");
+}
+
 bool known(int t) { return t == kF32 || t == kBF16 || t == kF16; }
 
 SeqPlan to_plan(const b2e_sequences* s, int rows) {
   SeqPlan p{};
+  check_extents({rows, s ? s->tokens : 0});
   if (s == nullptr) {  // one token a sequence, row i in state row i
     p.seqs = p.tokens = p.state_rows = rows;
     p.longest = rows > 0 ? 1 : 0;
     return p;
   }
   B2E_CHECK(s->seqs >= 0 && s->tokens >= 0 && s->state_rows >= 0 && s->longest >= 0, kErrInvalid, "negative plan sizes");
+  B2E_CHECK(s->seqs <= kMaxSeqs, kErrInvalid, "a plan has at most 2^30 sequences");
   B2E_CHECK(s->starts != nullptr || (s->tokens == s->seqs), kErrInvalid, "a plan without starts has one token a sequence");
   B2E_CHECK(s->slots != nullptr || s->seqs <= s->state_rows, kErrInvalid, "more sequences than state rows");
   B2E_CHECK(s->longest <= s->tokens, kErrInvalid, "the longest sequence has more tokens than the plan");
@@ -49,7 +57,7 @@ ScanParams to_scan(const b2e_sequences* plan, const b2e_scan_args* a) {
   B2E_CHECK(a != nullptr, kErrInvalid, "null scan arguments");
   B2E_CHECK(a->rows >= 0 && a->heads > 0 && a->size > 0 && a->state > 0, kErrInvalid, "scan sizes must be positive");
   B2E_CHECK(a->state <= kScanMaxState, kErrInvalid, "mamba2_scan: state columns must be in 1..256");
-  B2E_CHECK((long long)a->heads * a->size <= 0x7fffffffLL && a->heads <= 65535, kErrInvalid, "mamba2_scan: too many channels");
+  B2E_CHECK((long long)a->heads * a->size <= kMaxExtent && a->heads <= 65535, kErrInvalid, "mamba2_scan: too many channels");
   B2E_CHECK(known(a->dtype), kErrInvalid, "unknown dtype");
   ScanParams p{};
   p.plan = to_plan(plan, a->rows);
@@ -105,6 +113,7 @@ int b2e_rms_norm_fp8(const void* x, int32_t x_dtype, int64_t ldx, const void* re
                      void* total, void* normed, void* stream) {
   return abi_call([&] {
     B2E_CHECK(rows >= 0 && cols > 0, kErrInvalid, "rms_norm_fp8: bad sizes");
+    check_extents({rows, cols});
     B2E_CHECK(known(x_dtype), kErrInvalid, "unknown dtype");
     B2E_CHECK(rows == 0 || (x && q && scale), kErrInvalid, "null operand");
     B2E_CHECK(!residual || r_dtype == x_dtype || r_dtype == kF32, kErrInvalid,
@@ -121,6 +130,7 @@ int b2e_quantize_fp8(const void* x, int32_t x_dtype, int64_t ldx, int32_t rows, 
                      float* scale, void* stream) {
   return abi_call([&] {
     B2E_CHECK(rows >= 0 && cols > 0, kErrInvalid, "quantize_fp8: bad sizes");
+    check_extents({rows, cols});
     B2E_CHECK(known(x_dtype), kErrInvalid, "unknown dtype");
     B2E_CHECK(rows == 0 || (x && q && scale), kErrInvalid, "null operand");
     B2E_CHECK(ldx >= cols && ldq >= cols, kErrInvalid, "a row stride is shorter than a row");
@@ -134,6 +144,7 @@ int b2e_quantize_fp8_weight(const void* w, int32_t w_dtype, int64_t ldw, int32_t
                             float* scale, void* stream) {
   return abi_call([&] {
     B2E_CHECK(rows > 0 && cols > 0 && rows <= 65535 * kFp8Group, kErrInvalid, "quantize_fp8_weight: bad sizes");
+    check_extents({cols});
     B2E_CHECK(known(w_dtype), kErrInvalid, "unknown dtype");
     B2E_CHECK(w && q && scale, kErrInvalid, "null operand");
     B2E_CHECK(ldw >= cols && ldq >= cols, kErrInvalid, "a row stride is shorter than a row");
@@ -146,6 +157,7 @@ int b2e_fp8_linear(const void* q, int64_t ldq, const float* scale, int32_t m, in
                    void* stream) {
   return abi_call([&] {
     B2E_CHECK(m >= 0 && n > 0 && k > 0, kErrInvalid, "fp8_linear: bad sizes");
+    check_extents({m, n, k});
     B2E_CHECK(known(y_dtype), kErrInvalid, "unknown dtype");
     B2E_CHECK(act == 0 || act == 1, kErrInvalid, "unknown activation");
     if (m == 0) return;
@@ -165,6 +177,7 @@ int b2e_causal_conv(const b2e_sequences* plan, float* window, const void* x, int
                     int64_t ldy, void* stream) {
   return abi_call([&] {
     B2E_CHECK(rows >= 0 && channels > 0 && taps >= 2 && taps <= 4, kErrInvalid, "causal_conv: 2 to 4 taps, positive sizes");
+    check_extents({channels});
     B2E_CHECK(known(dtype), kErrInvalid, "unknown dtype");
     B2E_CHECK(act == 0 || act == 1, kErrInvalid, "unknown activation");
     ConvParams p{};

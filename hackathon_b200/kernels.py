@@ -156,6 +156,7 @@ def cast_linear(x, weight, bias=None, relu: bool = False, err=None):
 
 # ------------------------------------------------------------ runs of tokens
 
+MAX_EXTENT = 2 ** 31 - 1024  # rows, columns, tokens or channels of a call (the kernels' indices are 32-bit, their offsets are not)
 FP8_GROUP = 128  # columns of a row (rows and columns of a weight's block) that share a scale
 
 
@@ -176,7 +177,8 @@ class SequenceBatch:
         lengths = [int(n) for n in lengths]
         assert all(n >= 0 for n in lengths), "lengths must not be negative"
         self.tokens = sum(lengths)
-        assert self.tokens < 2 ** 31 and len(lengths) < 2 ** 31, "a batch has less than 2^31 tokens"
+        assert self.tokens <= MAX_EXTENT, "a batch has at most 2^31 - 1024 tokens"
+        assert len(lengths) <= 2 ** 30, "a batch has at most 2^30 sequences"
         if slots is not None:
             slots = [int(s) for s in slots]
             assert len(slots) == len(lengths), f"{len(slots)} slots for {len(lengths)} sequences"
@@ -229,6 +231,10 @@ def _call(name: str, device, *args) -> None:
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc)
+
+
+def _extents(*sizes: int) -> None:
+    assert max(sizes) <= MAX_EXTENT, f"sizes are at most 2^31 - 1024, got {max(sizes)}"
 
 
 def _at(t) -> Optional[int]:
@@ -303,6 +309,7 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-5, keep_norm: bo
     assert x.dim() == 2 and x.shape[1] > 0, f"x must be (rows, cols), got {tuple(x.shape)}"
     xt = _float(x, "x")
     rows, cols = x.shape
+    _extents(rows, cols)
     rt, ldr = xt, 0
     if residual is not None:
         assert residual.shape == x.shape, f"residual must be {tuple(x.shape)}, got {tuple(residual.shape)}"
@@ -327,9 +334,10 @@ def quantize_fp8(x):
     """e4m3 values of x (rows, cols) and the scale of each 128 columns of a row, (rows, ceil(cols / 128))."""
     assert x.dim() == 2 and x.shape[1] > 0, f"x must be (rows, cols), got {tuple(x.shape)}"
     xt = _float(x, "x")
+    rows, cols = x.shape
+    _extents(rows, cols)
     _on_gpu(x, "x")
     x, ldx = _rows(x)
-    rows, cols = x.shape
     q, groups = _empty8(rows, cols, x.device)
     scale = torch.empty(rows, groups, dtype=torch.float32, device=x.device)
     if rows:
@@ -341,9 +349,10 @@ def quantize_fp8_weight(weight):
     """e4m3 values of a weight (out, in) and the scale of each 128 x 128 block, (ceil(out / 128), ceil(in / 128))."""
     assert weight.dim() == 2 and weight.numel() > 0, f"weight must be (out, in), got {tuple(weight.shape)}"
     wt = _float(weight, "weight")
+    rows, cols = weight.shape
+    _extents(rows, cols)
     _on_gpu(weight, "weight")
     weight, ldw = _rows(weight)
-    rows, cols = weight.shape
     q, groups = _empty8(rows, cols, weight.device)
     scale = torch.empty(-(-rows // FP8_GROUP), groups, dtype=torch.float32, device=weight.device)
     _call("b2e_quantize_fp8_weight", weight.device, _at(weight), wt, ldw, rows, cols, _at(q), -(-cols // 16) * 16, _at(scale))
@@ -364,6 +373,7 @@ def fp8_linear(q, scale, wq, wscale, bias=None, relu: bool = False, out_dtype=to
     assert q.dtype == wq.dtype == torch.float8_e4m3fn, f"q and wq must be float8_e4m3fn, got {q.dtype} and {wq.dtype}"
     m, k = q.shape
     n, g = wq.shape[0], -(-k // FP8_GROUP)
+    _extents(m, n, k)
     dev = q.device
     _operand(scale, torch.float32, (m, g), "scale", dev)
     _operand(wscale, torch.float32, (-(-n // FP8_GROUP), g), "wscale", dev)
@@ -420,6 +430,7 @@ def causal_conv(window, x, weight, bias=None, seqs: Optional[SequenceBatch] = No
     _operand(weight, torch.float32, (ch, taps), "weight", dev)
     bias = _vector(bias, ch, "bias", dev)
     rows = x.shape[0]
+    _extents(rows, ch)
     plan, tokens = _plan(seqs, rows, window, "window")
     _on_gpu(window, "window")
     y = _out(x, rows, tokens)
@@ -455,6 +466,7 @@ def mamba2_scan(ssm, x, b, c, dt, a, seqs: Optional[SequenceBatch] = None, d=Non
     dev = ssm.device
     assert x.dim() == 3, f"x must be (rows, {h}, {p}), got {tuple(x.shape)}"
     rows, dtype = x.shape[0], x.dtype
+    _extents(rows, h * p)
     xt = _float(x, "x")
     _operand(x, dtype, (rows, h, p), "x", dev)
     if z is not None:

@@ -226,8 +226,10 @@ B2E_API int b2e_linear_static(const void* x, int32_t x_dtype, int32_t m, int32_t
  * symbol's whole run of tokens in one call and leave its state where as many
  * single steps would. Device pointers; row strides (ld*) in elements; sums,
  * statistics, scales and states are float32; dtype is B2E_DTYPE_* of the
- * activations. A call works on the current device and allocates nothing; make the
- * first one on each device before any stream capture (it looks the error word up).
+ * activations. Rows, columns, tokens, channels and heads * size are at most
+ * 2^31 - 1024 and sequences 2^30 (offsets may be larger). A call works on the
+ * current device and allocates nothing; make the first one on each device before any
+ * stream capture (it looks the error word up).
  *
  * Plan of a packed batch: sequence i is rows [starts[i], starts[i + 1]) of the
  * operands (starts[0] = 0, starts[seqs] = tokens) and row slots[i] of the state
