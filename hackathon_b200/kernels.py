@@ -303,8 +303,9 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-5, keep_norm: bo
     v = x + residual; n = v / sqrt(mean(v^2) + eps) * weight, all in float32; each 128
     columns of a row get scale = max(max|n| / 448, 2^-100) and q = e4m3(n / scale).
     ``total`` is v in the residual's type (x's or float32), the next layer's residual;
-    ``keep_norm`` adds n in x's type, for the projections that stay in float32. A NaN or
-    an infinity makes its whole row NaN, as the formula does.
+    ``keep_norm`` adds n in x's type, for the projections that stay in float32. As the
+    formula has it, a NaN makes its whole row NaN; an infinity makes its group of 128 NaN
+    and the rest of its row 0. Squares may leave float32's range.
     """
     assert x.dim() == 2 and x.shape[1] > 0, f"x must be (rows, cols), got {tuple(x.shape)}"
     xt = _float(x, "x")

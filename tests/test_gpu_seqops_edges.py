@@ -9,7 +9,7 @@ import torch
 from hackathon_b200 import _lib as L
 from hackathon_b200 import kernels as K
 from tests import seqops_ref as R
-from tests.test_gpu_seqops import DEV, PAIRS, TYPES, gen, ids, rnd, scan_inputs
+from tests.test_gpu_seqops import DEV, PAIRS, TYPES, check_q, gen, ids, norm_ref, rnd, scan_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -202,3 +202,49 @@ def test_split_sequences_among_others(dt, lengths):
     R.close(y, want, R.scan_tol(want, ymag, steps, dt, PAIRS[dt]) + 4 * 2.0 ** -22 * want.abs(), "y")
     R.close(inp["ssm"], ssm, R.scan_tol(ssm, smag, steps, torch.float32), "ssm")
     assert K.device_error() == 0
+
+
+# ------------------------------------------------- values at the ends of their types
+
+
+def normed_rows(x, eps, out):
+    """The rows' norm and its 8 bits against 64 bits."""
+    v, n, scale = norm_ref(x, None, None, eps)
+    check_q(out.q, out.scale, n, scale)
+    R.close(out.normed, n, R.rounding(n, x.dtype) + 2.0 ** -18 * n.abs(), "normed")
+
+
+@pytest.mark.parametrize("dt", TYPES[:2], ids=ids[:2])
+@pytest.mark.parametrize("cols", [256, 250, 1000, 1024, 4096, 8192, 9000])
+def test_rms_norm_squares_beyond_float32(dt, cols):
+    """Rows whose squares overflow or vanish, alone and beside ordinary ones."""
+    x = rnd(gen(80), 9, cols)
+    x *= torch.tensor([1.0, 1e19, 1e25, 2.0 ** 124 / 8, 1e-19, 1e-25, 1e-37, 1.0, 1.0], device=DEV)[:, None]
+    x[7, 3] = 3e38   # one value's square overflows
+    x[8, 5:] = 1e-30  # five values' squares outweigh the rest
+    x = x.clamp(-3.3e38, 3.3e38).to(dt)
+    for rows in (x, x[3:4].contiguous(), x[:0]):
+        normed_rows(rows, 0.0, K.rms_norm_fp8(rows, eps=0.0, keep_norm=True))
+        normed_rows(rows, 1e-5, K.rms_norm_fp8(rows, eps=1e-5, keep_norm=True))
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=ids)
+@pytest.mark.parametrize("cols", [256, 250, 1024, 4096])
+def test_rms_norm_rows_that_are_not_finite(dt, cols):
+    """A NaN makes its row NaN; an infinity its group, and the rest of its row zero; other rows keep their bits."""
+    x = rnd(gen(81), 6, cols).to(dt)
+    x[1, 5] = float("nan")
+    x[2, 7], x[3, cols - 1], x[4, 0], x[4, 1] = float("inf"), float("-inf"), float("inf"), float("nan")
+    out = K.rms_norm_fp8(x, keep_norm=True)
+    q, groups = out.q.float(), -(-cols // 128)
+    for row in (1, 4):
+        assert q[row].isnan().all() and out.scale[row].isnan().all() and out.normed[row].isnan().all()
+    for row, at in ((2, 7), (3, cols - 1)):
+        g = at // 128
+        assert q[row, g * 128:(g + 1) * 128].isnan().all() and out.scale[row, g].isnan()
+        assert out.normed[row, at].isnan() and int(out.normed[row].isnan().sum()) == 1
+        others = [i for i in range(groups) if i != g]
+        rest = [i for i in range(cols) if i // 128 != g]
+        assert not q[row, rest].any() and (out.scale[row, others] == 2.0 ** -100).all() and not out.normed[row, rest].any()
+    clean = K.rms_norm_fp8(x[[0, 5]].contiguous(), keep_norm=True)
+    assert torch.equal(q[[0, 5]], clean.q.float()) and torch.equal(out.scale[[0, 5]], clean.scale) and torch.equal(out.normed[[0, 5]], clean.normed)
