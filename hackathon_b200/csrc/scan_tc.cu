@@ -856,14 +856,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     if (!ok && lane == 0) failed();
   }
-  // log of the segment's decay, for the join: the same float32 sums, segment-wide
+  // log of the segment's decay, for the join: pairs as in the chunks, with the library's
+  // softplus, which this small part of the work can afford. Below e^-200 a decay is zero
+  // in float32; the bound keeps infinite steps (and no NaN) out of the pairs.
   if (ENDS && warp >= 20 && warp < 22) {
     const int head = h0 + warp - 20;
     if (head < p.heads) {
       Pair s{0.f, 0.f};
       for (int i = t.first + lane; i < end; i += 32) {
         const float raw = p.dt[(long long)i * p.lddt + head], dt = p.softplus ? softplusf_(raw) : raw;
-        s = add(s, {p.a[head] * dt, 0.f});
+        float x = p.a[head] * dt;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(-200.f));
+        s = add(s, {x, 0.f});
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s = add(s, {__shfl_xor_sync(0xffffffffu, s.hi, o), __shfl_xor_sync(0xffffffffu, s.lo, o)});

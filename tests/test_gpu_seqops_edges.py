@@ -248,3 +248,17 @@ def test_rms_norm_rows_that_are_not_finite(dt, cols):
         assert not q[row, rest].any() and (out.scale[row, others] == 2.0 ** -100).all() and not out.normed[row, rest].any()
     clean = K.rms_norm_fp8(x[[0, 5]].contiguous(), keep_norm=True)
     assert torch.equal(q[[0, 5]], clean.q.float()) and torch.equal(out.scale[[0, 5]], clean.scale) and torch.equal(out.normed[[0, 5]], clean.normed)
+
+
+# ------------------------------------------------- decay rates at the ends of float32
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=ids)
+@pytest.mark.parametrize("lengths", [[1, 1, 1], [300, 200, 40], [1500], [2, 1300, 700]], ids=["steps", "whole", "one split", "split"])
+def test_scan_with_extreme_rates(dt, lengths):
+    """Rates of minus infinity, of 1e30 and of zero: a state that is set anew with every token, or only added to."""
+    inp = scan_inputs(90, len(lengths), sum(lengths), 5, 64, 128, dt, True)
+    inp["a"] = torch.tensor([float("-inf"), -1e30, -3e38, -1.0, 0.0], device=DEV)
+    before = inp["ssm"].clone()
+    y = scan(inp, K.SequenceBatch(lengths, device=DEV))
+    against_recurrence(inp, before, y, lengths, PAIRS[dt])
