@@ -262,3 +262,97 @@ def test_scan_with_extreme_rates(dt, lengths):
     before = inp["ssm"].clone()
     y = scan(inp, K.SequenceBatch(lengths, device=DEV))
     against_recurrence(inp, before, y, lengths, PAIRS[dt])
+
+
+# ------------------------------------------------- offsets beyond 2^31 elements
+
+
+def need_memory(gib):
+    if torch.cuda.mem_get_info(DEV)[0] < gib << 30:
+        pytest.skip(f"needs {gib} GB of device memory")
+
+
+ROWS, STRIDE = 40, 2 ** 26 + 128  # the last rows start beyond 2^31 elements
+
+
+def far(base, like, at):
+    """The rows of `like` in rows STRIDE elements apart."""
+    flat = like.reshape(ROWS, -1)
+    view = base.as_strided(flat.shape, (STRIDE, 1), at)
+    view.copy_(flat)
+    return view.unflatten(1, like.shape[1:])
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=ids)
+@pytest.mark.parametrize("lengths", [[ROWS], [1] * ROWS, [9, 0, 31]], ids=["whole", "steps", "two"])
+def test_rows_far_apart(dt, lengths):
+    """Row strides that put the last rows beyond 2^31 elements: the packed operands' bits."""
+    need_memory(48)
+    h, p, n = 4, 64, 128
+    base = torch.empty(ROWS * STRIDE, dtype=dt, device=DEV)
+    steps = base if dt == torch.float32 else torch.empty(ROWS * STRIDE, dtype=torch.float32, device=DEV)
+    inp = scan_inputs(100, len(lengths), ROWS, h, p, n, dt, True)
+    wide = {k: far(base, inp[k], 512 * i) for i, k in enumerate(("x", "b", "c", "z"))}
+    wide["dt"] = far(steps, inp["dt"], 4096)
+    wide = {**inp, **wide, "ssm": inp["ssm"].clone()}
+    plan = K.SequenceBatch(lengths, device=DEV)
+    assert torch.equal(scan(wide, plan), scan(inp, plan)) and torch.equal(wide["ssm"], inp["ssm"])
+
+    x, flat = wide["x"].flatten(1), inp["x"].flatten(1)
+    assert x.stride(0) == STRIDE
+    for a, b in zip(K.rms_norm_fp8(x, residual=x), K.rms_norm_fp8(flat, residual=flat)):
+        assert a is b is None or torch.equal(a.float(), b.float())
+    for at in (x, x[:, 1:]):
+        for a, b in zip(K.quantize_fp8(at) + K.quantize_fp8_weight(at), K.quantize_fp8(at.contiguous()) + K.quantize_fp8_weight(at.contiguous())):
+            assert torch.equal(a.float(), b.float())
+    w = rnd(gen(101), h * p, 4)
+    win = rnd(gen(102), len(lengths), h * p, 3)
+    other = win.clone()
+    assert torch.equal(K.causal_conv(win, x, w, None, plan, silu=True), K.causal_conv(other, flat, w, None, plan, silu=True))
+    assert torch.equal(win, other) and K.device_error() == 0
+
+
+@pytest.mark.parametrize("m", [ROWS, 3])
+def test_projection_rows_far_apart(m):
+    need_memory(16)
+    g = gen(103)
+    q, scale = K.quantize_fp8(rnd(g, ROWS, 512))
+    wq, wscale = K.quantize_fp8_weight(rnd(g, ROWS, 512))
+    base = torch.empty(ROWS * STRIDE, dtype=torch.uint8, device=DEV)
+    fq, fw = (far(base, t.view(torch.uint8), at).view(torch.float8_e4m3fn) for t, at in ((q, 0), (wq, 1024)))
+    assert torch.equal(K.fp8_linear(fq[-m:], scale[-m:], fw, wscale), K.fp8_linear(q[-m:], scale[-m:], wq, wscale))
+    assert K.device_error() == 0
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("lengths", [[20, 30], [1, 1], [700, 2]], ids=["whole", "steps", "split"])
+@pytest.mark.parametrize("rows,n", [(40000, 128), (160000, 30)])
+def test_state_tables_beyond_32_bits(dt, lengths, rows, n):
+    """States behind 2^31 values of their table."""
+    need_memory(24)
+    h, p = 8, 64
+    inp = scan_inputs(104, 2, sum(lengths), h, p, n, dt, False)
+    table = torch.zeros(rows, h, p, n, device=DEV)
+    slots = [rows - 1, rows - 3]
+    table[slots] = inp["ssm"]
+    want = scan(inp, K.SequenceBatch(lengths, device=DEV))
+    y = scan({**inp, "ssm": table}, K.SequenceBatch(lengths, slots, device=DEV))
+    assert torch.equal(y, want) and torch.equal(table[slots], inp["ssm"])
+    assert not table[0].any() and not table[rows - 2].any()
+    assert K.device_error() == 0
+
+
+@pytest.mark.parametrize("lengths", [[20, 30], [1, 1]], ids=["prompt", "steps"])
+@pytest.mark.parametrize("ch", [4352, 4351])
+def test_windows_beyond_32_bits(lengths, ch):
+    need_memory(24)
+    rows = 170000
+    g = gen(105)
+    x, w, small = rnd(g, sum(lengths), ch), rnd(g, ch, 4), rnd(g, 2, ch, 3)
+    table = torch.zeros(rows, ch, 3, device=DEV)
+    slots = [rows - 1, rows - 3]
+    table[slots] = small
+    want = K.causal_conv(small, x, w, None, K.SequenceBatch(lengths, device=DEV))
+    y = K.causal_conv(table, x, w, None, K.SequenceBatch(lengths, slots, device=DEV))
+    assert torch.equal(y, want) and torch.equal(table[slots], small)
+    assert not table[0].any() and not table[rows - 2].any()
