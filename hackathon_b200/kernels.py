@@ -20,6 +20,7 @@ does not have: ``rms_norm_fp8``, ``fp8_linear`` with its quantisers,
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import struct
 from typing import NamedTuple, Optional, Sequence
 
@@ -160,6 +161,13 @@ MAX_EXTENT = 2 ** 31 - 1024  # rows, columns, tokens or channels of a call (the 
 FP8_GROUP = 128  # columns of a row (rows and columns of a weight's block) that share a scale
 
 
+def _integers(values, name: str) -> list:
+    try:
+        return [operator.index(v) for v in values]
+    except TypeError:
+        raise AssertionError(f"{name} must be integers") from None
+
+
 class SequenceBatch:
     """Plan of a packed batch of sequences, kept for every call on that batch.
 
@@ -174,18 +182,18 @@ class SequenceBatch:
 
     def __init__(self, lengths: Sequence[int], slots: Optional[Sequence[int]] = None, *,
                  state_rows: Optional[int] = None, device=None):
-        lengths = [int(n) for n in lengths]
+        lengths = _integers(lengths, "lengths")
         assert all(n >= 0 for n in lengths), "lengths must not be negative"
         self.tokens = sum(lengths)
         assert self.tokens <= MAX_EXTENT, "a batch has at most 2^31 - 1024 tokens"
         assert len(lengths) <= 2 ** 30, "a batch has at most 2^30 sequences"
         if slots is not None:
-            slots = [int(s) for s in slots]
+            slots = _integers(slots, "slots")
             assert len(slots) == len(lengths), f"{len(slots)} slots for {len(lengths)} sequences"
             assert len(set(slots)) == len(slots), "slots must be distinct"
             assert all(s >= 0 for s in slots), "slots must not be negative"
         need = (max(slots) + 1 if slots else 0) if slots is not None else len(lengths)
-        self.state_rows = need if state_rows is None else int(state_rows)
+        self.state_rows = need if state_rows is None else _integers([state_rows], "state_rows")[0]
         assert need <= self.state_rows < 2 ** 31, f"slots reach row {need - 1} of {self.state_rows} state rows"
         self.lengths = tuple(lengths)
         self.longest = max(lengths, default=0)

@@ -2,6 +2,7 @@
 
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
@@ -83,3 +84,17 @@ def test_c_abi_refuses_sizes_beyond_32_bit_indices(n):
     many_seqs = C.byref(_lib.SequencesC(P, None, None, 2 ** 30 + 1, 5, 2 ** 31 - 1, 5))
     assert lib.b2e_causal_conv(many_seqs, P, P, 0, 1, 5, 1, P, None, 4, 0, P, 1, None) == -1
     assert "2^30" in lib.b2e_last_error().decode()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(lengths=[2.9, 1]), dict(lengths=torch.tensor([2.0, 1.0])), dict(lengths=[2, 1], slots=[0, 1.5]),
+    dict(lengths=[2, 1], state_rows=2.5), dict(lengths=["2"]),
+])
+def test_plan_refuses_what_is_not_a_whole_number(kw):
+    with pytest.raises(AssertionError, match="must be integers"):
+        K.SequenceBatch(**kw, device="cpu")
+
+
+def test_plan_takes_integers_of_other_kinds():
+    b = K.SequenceBatch(torch.tensor([3, 0, 2]), np.array([4, 0, 1]), state_rows=np.int64(5), device="cpu")
+    assert (b.lengths, b.slots, b.state_rows, b.tokens) == ((3, 0, 2), (4, 0, 1), 5, 5)
