@@ -2,6 +2,8 @@
 chunk, plans and extents at their limits, values at the ends of their types."""
 
 import ctypes as C
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -356,3 +358,26 @@ def test_windows_beyond_32_bits(lengths, ch):
     y = K.causal_conv(table, x, w, None, K.SequenceBatch(lengths, slots, device=DEV))
     assert torch.equal(y, want) and torch.equal(table[slots], small)
     assert not table[0].any() and not table[rows - 2].any()
+
+
+# ------------------------------------------------- the integration guide's example
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=ids)
+def test_example_of_the_guide_runs(dt):
+    """The layer in INTEGRATION.md, as it stands there."""
+    text = (Path(__file__).resolve().parent.parent / "INTEGRATION.md").read_text()
+    code = next(b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "mamba2_scan(" in b)
+    g, heads, size, bc, hid, tokens, rows = gen(110), 4, 64, 128, 256, 666, 16
+    inner = heads * size
+    env = dict(torch=torch, inner=inner, bc=bc, heads=heads, size=size, u=rnd(g, tokens, hid).to(dt), residual=rnd(g, tokens, hid).to(dt),
+               norm_weight=torch.ones(hid, device=DEV), weight=rnd(g, 2 * inner + 2 * bc, hid) * hid ** -0.5,
+               window=torch.zeros(rows, inner + 2 * bc, 3, device=DEV), conv_weight=rnd(g, inner + 2 * bc, 4), conv_bias=rnd(g, inner + 2 * bc),
+               dt_weight=rnd(g, heads, hid) * hid ** -0.5, dt_bias=rnd(g, heads), ssm=torch.zeros(rows, heads, size, bc, device=DEV),
+               a=-torch.ones(heads, device=DEV), d=torch.ones(heads, device=DEV))
+    exec(code, env)
+    assert env["y"].shape == (tokens, heads, size) and env["y"].dtype == dt and env["y"].isfinite().all() and env["y"].any()
+    stepped = [7, 3, 12]
+    assert all(env["ssm"][r].any() and env["window"][r].any() for r in stepped)
+    assert not any(env["ssm"][r].any() for r in range(rows) if r not in stepped)
+    assert K.device_error() == 0
