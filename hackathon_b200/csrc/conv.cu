@@ -16,8 +16,11 @@
 // four times the tokens), where half the bytes meet the same arithmetic: 39 us
 // without SiLU. Sixteen tokens in flight in shared memory instead of four in
 // registers changed nothing (46 to 48 us); tiles of 24 or 64 tokens were slower.
-// Single tokens, 4096 x 768 float32: 18.4 us with part of the windows in L2, 24.6
-// out of a cold cache (5.1 TB/s).
+// Single tokens, 4096 x 768 float32, 101 MB: 17.2 us with part of the windows in L2,
+// 21 to 25 out of a cold cache (4.0 to 4.8 TB/s). Bound by latency and sectors rather
+// than HBM (a warp waits 7.4 cycles an instruction for memory, DRAM is at a third): a
+// lane's windows start 48 bytes from its neighbour's, so that an access touches
+// sectors that two others touch again.
 #include <algorithm>
 
 #include "packed.cuh"

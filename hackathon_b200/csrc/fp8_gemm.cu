@@ -14,12 +14,13 @@
 //  - rows kernel: M = 128 activation rows (a thread's TMEM lane is a row, so both
 //    scales are one scalar a thread and group), N = BN output features;
 //    persistent CTAs. Bound by the exchange of the accumulators: a group of BN =
-//    256 takes the tensor cores 515 cycles, and its sums, read from TMEM and
-//    scaled by eight warps (128 FMAs a thread), about 800. 18944 x 4096 x 4096 to
-//    bf16 takes 322 us (1.97 PFLOP/s), 10000 x 4096 x 2048 101 us (1.66), where a
-//    last round of whole tiles over the SMs would leave most of them idle: tiles
-//    that would are taken in halves (104 us without; 4096 x 256 x 1280 13.5 us
-//    for 14.8, 300 x 2048 x 8448 18.0 for 19.4).
+//    256 keeps the tensor cores busy for 515 cycles of some 1,070 at 10000 x 4096 x
+//    2048 (48%, starts and stores of the tiles included); its sums are read from TMEM
+//    and scaled by eight warps, 128 scalar FMAs a thread.
+//    18944 x 4096 x 4096 to bf16 takes 322 us (1.97 PFLOP/s), 10000 x 4096 x 2048 103
+//    us (1.63), where a last round of whole tiles over the SMs would leave most of
+//    them idle: tiles that would are taken in halves (104 us without when 101 with;
+//    4096 x 256 x 1280 13.5 us for 14.8, 300 x 2048 x 8448 18.0 for 19.4).
 //  - few-rows kernel, where there are not tiles for every SM: M = 128 output
 //    features, N = BR rows (16, 32 or 64; a grid of them above 64); the groups are
 //    shared out over a cluster of up to 8 CTAs, whose float32 sums meet through

@@ -5,7 +5,8 @@
 //   dt = softplus(dt);  h <- exp(a dt) h + (dt x) b^T;  y = (h c + d x) silu(z)
 //
 // h is [size, state] float32 a (sequence, head), x [size], b and c [state], dt, a
-// and d scalars of the head. Everything is held in float32; y is rounded once.
+// and d scalars of the head. In this file's kernels everything is held in float32 and
+// y is rounded once.
 //
 // Here: the single-token kernels, the recurrence kernel that walks a sequence
 // token by token with the state in registers (any type and size), the join of a
@@ -164,12 +165,16 @@ __global__ void __launch_bounds__(256) k_scan_step_any(const ScanParams p) {
 // two where only the state is wanted. P is multiplied into H when it leaves
 // [2^-12, 2^12] (P and the token's decay one after the other, as h would have
 // been multiplied) and at the end, so dt x b has 2^12 of headroom less than
-// float32's range, and a decay is rounded into P as it would be into h.
+// float32's range. A decay is rounded into P as it would be into h, and 1 / P is the
+// hardware's reciprocal (one ulp): the outputs are 2.1e-7 from 64 bits (relative
+// 2-norm, 64 sequences of 10000 tokens in all).
 //
-// Bound by the FP32 pipe (two elements an instruction, two cycles each) and, a
-// third of the issue slots, the exchange of row sums. The layout keeps shared
-// memory off that path: a token costs a thread 2 J + R / 4 vectors. 64 sequences of
-// 10000 tokens in all, 8 heads of 64 x 128, float32: 195 us; 220 with three
+// That batch, 8 heads of 64 x 128, float32: 187 us, of which the main pass is 139, the
+// pass for the segments' contributions 44 and their join 13. Bound by latency and
+// issue, with 13 warps on an SM: 57% of the issue slots are taken and the FP32 pipe is
+// busy half of the time that an SM is; an SM is idle for a quarter of the main pass,
+// behind its last segment. The layout keeps shared memory off that path: a token costs
+// a thread 2 J + R / 4 vectors. With a join 8 us slower than now: 195 us as it is, 220 with three
 // operations, 204 with four rows a thread, 294 with two rows and 32 columns, where
 // shared memory bound it. Tokens are staged in blocks of 16, the next block by
 // cp.async while one is computed where the operands are float32 vectors.
@@ -550,7 +555,7 @@ ScanWork scan_work(const ScanParams& p, int seg) {
 // of 128 tokens: rounded down for the recurrence kernel, whose CTAs queue, up for
 // the chunked one, where one CTA too many is a second wave. 64 sequences of 10000
 // tokens in all (up to 700), 8 heads, float32: 288 us whole, 195 us split in 128
-// tokens, 254 us in 256.
+// tokens (187 with today's join), 254 us in 256.
 int scan_segment(const ScanParams& p) {
   if (single_tokens(p)) return 0;
   const bool tc = scan_tc_eligible(p);

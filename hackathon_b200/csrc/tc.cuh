@@ -92,13 +92,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t* r) {
       "r"(t)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::B2E_I16(r, 0),
-      B2E_I16(r, 16), "r"(t)
-      : "memory");
-}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Register values that an asynchronous TMEM load filled: keeps their uses below

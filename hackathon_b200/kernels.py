@@ -340,7 +340,9 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-5, keep_norm: bo
 
 
 def quantize_fp8(x):
-    """e4m3 values of x (rows, cols) and the scale of each 128 columns of a row, (rows, ceil(cols / 128))."""
+    """e4m3 values of x (rows, cols) and the scale of each 128 columns of a row, (rows, ceil(cols / 128)).
+
+    As ``rms_norm_fp8`` has them of n. A NaN makes its group of 128 NaN; so does an infinity."""
     assert x.dim() == 2 and x.shape[1] > 0, f"x must be (rows, cols), got {tuple(x.shape)}"
     xt = _float(x, "x")
     rows, cols = x.shape
@@ -462,13 +464,22 @@ def mamba2_scan(ssm, x, b, c, dt, a, seqs: Optional[SequenceBatch] = None, d=Non
     y = (sum_c c * ssm + d x) * silu(z). ``ssm`` (state rows, heads, size, state) float32 is
     updated IN PLACE; rows of no sequence, and of empty ones, stay bit for bit. ``x``, ``z``
     (rows, heads, size), ``b``, ``c`` (rows, state), state up to 256, all of one type; ``dt``
-    (rows, heads), ``a`` and ``d`` (heads,) float32. The state and all sums are float32 and y
-    is rounded once to x's type. Without ``seqs`` each row is one token of that row of
-    ``ssm``, as in ``mamba2_step``. Rows behind the batch's tokens are not read and give zeros.
+    (rows, heads), ``a`` and ``d`` (heads,) float32. Without ``seqs`` each row is one token of
+    that row of ``ssm``, as in ``mamba2_step``. Rows behind the batch's tokens are not read and
+    give zeros.
+
+    The state and all sums are float32 and y is rounded once to x's type. In bf16 prompts with
+    heads of 64 and states of 64 or 128, which run in chunks of 128 tokens on the tensor cores,
+    two operands of y are rounded to bf16 as well: the weights of a chunk's pairs of tokens and
+    the copy of the state that c multiplies. A term of y is then within 2^-8 of its value, and y
+    about 1.35 times as far from the formula as its own rounding takes it; the state is not
+    affected.
 
     A value that is not finite stays in its own sequence and reaches no earlier token; of x, it
-    makes its row's y NaN from its token on. ``a`` is meant to be at most zero: with one above,
-    bf16 prompts (chunks of 128 tokens) overflow where the sum of a t over a chunk passes 88.
+    makes its row's y NaN from its token on; bf16 prompts may have NaN where the formula has an
+    infinity. ``a`` is meant to be at most zero: with one above, those chunks overflow where the
+    sum of a t over one passes 88. Prompts of other types hold the state relative to the product
+    of its decays, which leaves t x b a headroom of 2^12 below float32's largest.
     """
     _scan_state_ok(ssm)
     nrows, h, p, n = ssm.shape

@@ -225,8 +225,8 @@ B2E_API int b2e_linear_static(const void* x, int32_t x_dtype, int32_t m, int32_t
  * No counterpart in the reference, which steps one token at a time: these take a
  * symbol's whole run of tokens in one call and leave its state where as many
  * single steps would. Device pointers; row strides (ld*) in elements; sums,
- * statistics, scales and states are float32; dtype is B2E_DTYPE_* of the
- * activations. Rows, columns, tokens, channels and heads * size are at most
+ * statistics, scales and states are float32 (b2e_mamba2_scan rounds two operands of
+ * y in bf16 prompts, as said there); dtype is B2E_DTYPE_* of the activations. Rows, columns, tokens, channels and heads * size are at most
  * 2^31 - 1024 and sequences 2^30 (offsets may be larger). A call works on the
  * current device and allocates nothing; make the first one on each device before any
  * stream capture (it looks the error word up).
@@ -290,8 +290,12 @@ B2E_API int b2e_causal_conv(const b2e_sequences* plan, float* window, const void
  * have rows of heads * size values, b and c of state (1..256), dt of heads
  * float32; d and z may be NULL. Long sequences in a small batch are split over
  * the device, which takes b2e_mamba2_scan_workspace() bytes (16-byte aligned, 0
- * and NULL where none is needed) for the same plan and arguments. y may not overlap an
- * input. a is meant to be at most 0: above, prompts in bf16 (chunks of 128 tokens) overflow
+ * and NULL where none is needed; at most two states a head for each 128 tokens) for
+ * the same plan and arguments; calls that may run at the same time, captured graphs
+ * among them, each have their own. y may not overlap an input. bf16 prompts with heads
+ * of 64 and states of 64 or 128 columns round the weights of token pairs and the copy
+ * of the state that c multiplies to bf16: a term of y is within 2^-8 of its value; the
+ * state is not affected. a is meant to be at most 0: above, prompts in bf16 (chunks of 128 tokens) overflow
  * where the sum of a t over a chunk passes 88. A value of x that is not finite makes its
  * row's y NaN from its token on. */
 typedef struct b2e_scan_args {
