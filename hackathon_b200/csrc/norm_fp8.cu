@@ -27,8 +27,9 @@ namespace {
 
 // The factor that brings a row's values where their squares are float32 numbers: 0,
 // none needed, for a mean square (and eps) between 2^-100 and the largest float32, or
-// NaN. 2^-100 of a row whose squares overflow leaves them between 2^-104 and 2^56.
-__device__ __forceinline__ float rescale(float ms) { return ms > 3.4028235e38f ? 0x1p-100f : ms < 0x1p-100f ? 0x1p100f : 0.f; }
+// NaN. Of 2^31 columns, squares that overflow together leave the largest between 2^-103
+// and 2^56, so their sum below 2^87; a mean below 2^-100 leaves the sum below 2^111.
+__device__ __forceinline__ float rescale(float ms) { return ms > 3.4028235e38f ? 0x1p-100f : ms < 0x1p-100f ? 0x1p90f : 0.f; }
 __device__ __forceinline__ float root(float ss, int cols, float eps, float up) { return up / sqrtf(ss / float(cols) + eps * up * up); }
 
 // max that keeps a NaN, so that a group holding one gets a NaN scale.

@@ -16,6 +16,11 @@ from tests.test_gpu_seqops import DEV, PAIRS, TYPES, check_q, gen, ids, norm_ref
 pytestmark = pytest.mark.gpu
 
 
+def need_memory(gib):
+    if torch.cuda.mem_get_info(DEV)[0] < gib << 30:
+        pytest.skip(f"needs {gib} GB of device memory")
+
+
 def scan(inp, seqs, **kw):
     return K.mamba2_scan(inp["ssm"], inp["x"], inp["b"], inp["c"], inp["dt"], inp["a"], seqs, d=inp["d"], z=inp["z"], **kw)
 
@@ -230,6 +235,18 @@ def test_rms_norm_squares_beyond_float32(dt, cols):
         normed_rows(rows, 1e-5, K.rms_norm_fp8(rows, eps=1e-5, keep_norm=True))
 
 
+def test_rms_norm_of_one_value_in_a_very_long_row():
+    """Its square, 2^-72, vanishes in the mean of 2^29, and is far from it when scaled for that mean."""
+    need_memory(16)
+    x = torch.zeros(1, 2 ** 29, dtype=torch.bfloat16, device=DEV)
+    x[0, 5] = 2.0 ** -36
+    out = K.rms_norm_fp8(x, eps=0.0, keep_norm=True)
+    want = 2.0 ** 14.5  # 2^-36 / sqrt(2^-72 / 2^29)
+    assert abs(float(out.normed[0, 5]) / want - 1) < R.half(torch.bfloat16) + 2.0 ** -18
+    assert abs(float(out.scale[0, 0]) * 448 / want - 1) < 2.0 ** -18 and float(out.q[0, 5]) == 448.0
+    assert int(out.normed.count_nonzero()) == 1
+
+
 @pytest.mark.parametrize("dt", TYPES, ids=ids)
 @pytest.mark.parametrize("cols", [256, 250, 1024, 4096])
 def test_rms_norm_rows_that_are_not_finite(dt, cols):
@@ -267,11 +284,6 @@ def test_scan_with_extreme_rates(dt, lengths):
 
 
 # ------------------------------------------------- offsets beyond 2^31 elements
-
-
-def need_memory(gib):
-    if torch.cuda.mem_get_info(DEV)[0] < gib << 30:
-        pytest.skip(f"needs {gib} GB of device memory")
 
 
 ROWS, STRIDE = 40, 2 ** 26 + 128  # the last rows start beyond 2^31 elements
